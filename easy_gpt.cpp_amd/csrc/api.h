@@ -391,14 +391,30 @@ int egpt_argmax(const float* logits, int32_t* out, void* scratch, int n_rows, in
 #define EGPT_ARGMAX_STATIC_MAX_ROWS 1024
 int egpt_argmax_static_init(void);
 int egpt_argmax_static(const float* logits, int32_t* out, int n_rows, int vocab, void* stream);
-// weights: scratch for n_rows * vocab floats.
+// min_p float32 [n_rows] or null: of what top-k and top-p keep, the tokens at least min_p times as likely as the most likely one (here
+// and below).  weights: scratch for n_rows * vocab floats.
 int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream);
+                const float* min_p, const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream);
 // The same in stages for wide vocabularies (several workgroups per row, then the selection on the tokens that can still
 // be kept); workspace: egpt_sample_workspace(n_rows, vocab) bytes of device memory.
 size_t egpt_sample_workspace(int n_rows, int vocab);
 int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                     const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream);
+                     const float* min_p, const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream);
+
+// ---- drafted tokens (attention_tree.hip, drafts.hip)
+// Attention for trees: operands as egpt_paged_attention; the last q_len[b] of a request's kv_len[b] tokens are its nodes.  visible int64
+// [n_tokens]: bit m of a node's number says that it reads node m.  window > 0: a node reads the tokens before the tree from place positions[t] -
+// window + 1 on.  n_pages: the caches' pages; a table's entry outside them is read as no page.  Any head size up to 256, any page size.
+int egpt_tree_attention_generic(const void* qkv, void* out, const void* k_cache, const void* v_cache, const int32_t* block_table, int table_width,
+                                int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
+                                const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,
+                                int dtype, void* stream);
+// path, accepted int32 [n_seqs][64], count int32 [n_seqs]
+int egpt_accept_drafts(const int32_t* tokens, const int32_t* parents, const int32_t* sampled, const int32_t* q_start, const int32_t* q_len, int n_seqs,
+                       int n_tokens, int32_t* path, int32_t* count, int32_t* accepted, void* stream);
+// k_cache [n_slabs][n_pages][nkv][page_size][dk], v_cache [n_slabs][n_pages][nkv][dv][page_size]; path int32 [n_seqs][path_width], ascending.
+int egpt_keep_drafts(void* k_cache, void* v_cache, const int32_t* block_table, int table_width, const int32_t* start, const int32_t* path, int path_width,
+                     const int32_t* count, int n_seqs, int n_slabs, int n_pages, int page_size, int nkv, int dk, int dv, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

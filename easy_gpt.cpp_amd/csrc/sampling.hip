@@ -6,6 +6,9 @@
 // kept mass.  Here the kept set is found without sorting, by radix selection on the bit patterns of the
 // weights (four passes of eight bits over the row, which stays in cache; masses are added in fixed point so
 // that no decision depends on the order of additions), and the draw walks the kept weights in index order.
+// A fourth cut that the reference does not have, min_p: of what the others keep, the tokens at least min_p times as
+// likely as the most likely one.  A weight is exp((x - max) / T), so that is a comparison with min_p itself: known before
+// the row is read, where the other thresholds have to be searched for.
 #include <mutex>
 
 #include "api.h"
@@ -374,6 +377,17 @@ constexpr float kNoTopBin = -10.5f;
 // A row with top-k whose candidates follow from the shares' maxima: nothing of it underflows, and there are k maxima.
 constexpr float kLeastExponent = -80.0f;
 
+// The least weight that min_p keeps (0: min_p cuts nothing; the most likely tokens weigh 1 and stay whatever it is).
+__device__ __forceinline__ float least_of(const float* __restrict__ min_p, int r) {
+    const float m = min_p ? min_p[r] : 0.f;
+    return m > 0.f ? fminf(m, 1.0f) : 0.f;               // (a NaN cuts nothing)
+}
+// A row that min_p alone cuts, at a weight of the top bins: its bound is known without the shares' maxima, and its candidates are listed by the pass
+// that would count the others'.
+__device__ __forceinline__ bool listed_by_least(int k, float p, float least, int vocab) {
+    return !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f) && top_bin_of(__float_as_uint(least)) < kTopBins;
+}
+
 // The k-th largest of a row's kSubPieces maxima (k <= kSubPieces; 256 threads, `mine` the maximum of thread t < kSubPieces).
 __device__ float bound_of_row(float mine, int k, float* s_sub /* [kSubPieces] */, unsigned int* s_bound) {
     const int t = threadIdx.x;
@@ -402,11 +416,12 @@ __device__ float bound_of_row(float mine, int k, float* s_sub /* [kSubPieces] */
 // back.  `first`: the thread's tokens begin + t, begin + t + 256 ..., kCollectAhead of them, on their way since the kernel began.
 constexpr int kCollectAhead = 20;
 __device__ void collect_candidates(const float* __restrict__ row, int begin, int n, const float (&first)[kCollectAhead], float mx, float inv_t,
-                                   float bound_t, float* __restrict__ ow, int32_t* __restrict__ oi, int* s_n /* [2], zeros */) {
-    // (expf may be off by a unit either way: 2^-18 below the bound is below every token that is not)
-    const float tight = expf(bound_t) * (1.0f - 3.8147e-6f);
+                                   float bound_t, float least, float* __restrict__ ow, int32_t* __restrict__ oi, int* s_n /* [2], zeros */) {
+    // (expf may be off by a unit either way: 2^-18 below the bound is below every token that is not.  `least` > 0: the bound is that weight,
+    // and nobody counts by its exponent)
+    const float tight = least > 0.f ? least : expf(bound_t) * (1.0f - 3.8147e-6f);
     const uint32_t bits = __float_as_uint(tight);
-    const float loose = top_bin_of(bits) < kTopBins ? __uint_as_float(bits & 0x7f800000u) : tight;
+    const float loose = least == 0.f && top_bin_of(bits) < kTopBins ? __uint_as_float(bits & 0x7f800000u) : tight;
     const float far = bound_t - 0.75f;                       // e^-0.75 < 1/2
     auto look = [&](float x, int j) {
         const float t = exponent_of(x, mx, inv_t);
@@ -443,7 +458,8 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
                                                           int32_t* __restrict__ list_count,
                                                           float* __restrict__ cand_w, int32_t* __restrict__ cand_idx,
                                                           unsigned int* __restrict__ piece_count,
-                                                          unsigned long long* __restrict__ piece_mass, int vocab) {
+                                                          unsigned long long* __restrict__ piece_mass, int vocab,
+                                                          const float* __restrict__ top_p, const float* __restrict__ min_p) {
     __shared__ __attribute__((aligned(16))) float s_sub[kSubPieces];
     __shared__ unsigned int s_bound;
     __shared__ int s_n[2];
@@ -457,7 +473,9 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
     const int piece = (vocab + kSamplePieces - 1) / kSamplePieces;
     const int begin = min(vocab, c * piece), n = min(vocab, begin + piece) - begin;
     // everything that can be asked for is asked for at once: what follows is a chain of waits otherwise
-    const bool may_list = temp > 0.f && by_count && k <= kSubPieces;
+    const float least = least_of(min_p, r);
+    const bool by_least = least > 0.f && listed_by_least(k, top_p[r], least, vocab);
+    const bool may_list = temp > 0.f && ((by_count && k <= kSubPieces) || by_least);
     float first[kCollectAhead], sub = 0.f;
     if (may_list) {
 #pragma unroll
@@ -465,7 +483,7 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
             const int j = threadIdx.x + 256 * i;
             first[i] = j < n ? row[begin + j] : -INFINITY;
         }
-        if (threadIdx.x < kSubPieces) sub = sub_val[r * kSubPieces + threadIdx.x];
+        if (!by_least && threadIdx.x < kSubPieces) sub = sub_val[r * kSubPieces + threadIdx.x];
     }
     const BestToken best = best_of_pieces(piece_val, piece_idx, r, threadIdx.x % kWave);
     if (c == 0 && threadIdx.x == 0) best_out[r] = best.index;
@@ -474,9 +492,10 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
     const float inv_t = 1.0f / fmaxf(temp, 1e-6f);
     if (may_list) {
         if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
-        const float bound_t = exponent_of(bound_of_row(sub, k, s_sub, &s_bound), mx, inv_t);
+        const float bound_t = by_least ? logf(least) : exponent_of(bound_of_row(sub, k, s_sub, &s_bound), mx, inv_t);
+        if (by_least) __syncthreads();                       // (s_n is zeros, for everybody; the bound's search waits as well)
         if (bound_t >= kLeastExponent && fabsf(mx) < INFINITY) {
-            collect_candidates(row, begin, n, first, mx, inv_t, bound_t, cand_w + static_cast<size_t>(r) * vocab,
+            collect_candidates(row, begin, n, first, mx, inv_t, bound_t, by_least ? least : 0.f, cand_w + static_cast<size_t>(r) * vocab,
                                cand_idx + static_cast<size_t>(r) * vocab, s_n);
             if (c == 0 && threadIdx.x == 0) listed[r] = 1;
             __syncthreads();
@@ -534,20 +553,21 @@ struct SamplePlan {
     int direct_piece;                   // without cuts: the piece that holds the drawn point, and what is left of it there
     unsigned long long direct_target;   // (top-p without top-k: the mass of the bins above `last`, from which its search goes on)
 };
+constexpr unsigned long long kAllPass = ~0ull;      // (in direct_target's place: nothing of the list is cut by top-p)
 struct SamplePlanSpace {
     unsigned int count[kSamplePieces][kTopBins + 1];
     unsigned long long mass[kSamplePieces][kTopBins + 1], bin_mass[kTopBins + 1];
     unsigned int bin_count[kTopBins + 1];
     int last, start[kSamplePieces + 1];
 };
-__device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, float u, const unsigned int* __restrict__ piece_count,
+__device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, float least, float u, const unsigned int* __restrict__ piece_count,
                                                   const unsigned long long* __restrict__ piece_mass, int vocab, SamplePlanSpace& space) {
     SamplePlan plan{kTopBins, 0, 0, 0, 0ull, -1, 0ull};
     const int t = threadIdx.x;
-    const bool by_count = k > 0 && k < vocab, by_mass = p > 0.f && p < 1.f;
+    const bool by_count = k > 0 && k < vocab, by_mass = p > 0.f && p < 1.f, by_least = least > 0.f;
     const unsigned int* counts = piece_count + static_cast<size_t>(r) * kSamplePieces * (kTopBins + 1);
     const unsigned long long* masses = piece_mass + static_cast<size_t>(r) * kSamplePieces * (kTopBins + 1);
-    if (!by_count && !by_mass) {
+    if (!by_count && !by_mass && !by_least) {
         // The pieces' masses are known, so the drawn point (in fixed point, of the whole row's mass) names its piece and what is
         // left of it inside that piece; the last kernel walks that piece alone.  (Every wavefront finds the same.)
         const int lane = t % kWave;
@@ -605,6 +625,7 @@ __device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, 
             for (int i = 0; i <= kTopBins; ++i) total += space.bin_mass[i];
             unsigned long long need = static_cast<unsigned long long>(static_cast<double>(p) * static_cast<double>(total));
             if (need == 0ull) need = 1ull;
+            if (!by_mass) need = ~0ull;                      // (min_p alone cuts)
             unsigned long long over = 0ull;
             for (int i = 0; i <= kTopBins; ++i) {
                 if (cum < need) {
@@ -615,6 +636,11 @@ __device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, 
             }
             space.bin_mass[0] = total;
             space.bin_mass[1] = over;
+            // below min_p's bin nothing is kept; the mass p is then not reached within the list, and all of it passes top-p
+            if (by_least && top_bin_of(__float_as_uint(least)) < last) {
+                last = top_bin_of(__float_as_uint(least));
+                space.bin_mass[1] = kAllPass;
+            }
         }
         space.last = last;
     }
@@ -654,7 +680,7 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
                                                              unsigned long long* __restrict__ row_mass,
                                                              int32_t* __restrict__ direct_piece,
                                                              unsigned long long* __restrict__ direct_target,
-                                                             int32_t* __restrict__ last_bin, int vocab) {
+                                                             int32_t* __restrict__ last_bin, int vocab, const float* __restrict__ min_p) {
     __shared__ int s_wave[4];
     __shared__ SamplePlanSpace s_plan;
     const int r = blockIdx.x, c = blockIdx.y;
@@ -667,12 +693,13 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
     const float* row = logits + static_cast<size_t>(r) * vocab;
     const float mx = row[best[r]];
     const float inv_t = 1.0f / fmaxf(temp, 1e-6f);
+    const float least = least_of(min_p, r);
     {
         const int k = top_k[r];
         const float p = top_p[r];
-        if (c > 0 && !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f)) return;      // no list is made without cuts
+        if (c > 0 && !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f) && !(least > 0.f)) return;      // no list is made without cuts
     }
-    SamplePlan plan = plan_of_row(r, c, top_k[r], top_p[r], uniform[r], piece_count, piece_mass, vocab, s_plan);
+    SamplePlan plan = plan_of_row(r, c, top_k[r], top_p[r], least, uniform[r], piece_count, piece_mass, vocab, s_plan);
     if (!(fabsf(mx) < INFINITY)) {                           // an infinity or nothing but NaN: the row's best token and no draw
         plan.total = 0;
         plan.last = plan.direct_piece = -1;
@@ -748,7 +775,7 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
 // iff the mass of the greater weights is below it: the same sets as the thresholds of select_by_count and
 // select_by_mass (ties whole).  Counts and fixed-point masses are integers, so nothing depends on an order; the
 // draw walks the kept weights in index order.  Returns the picked position in the list or -1 (every thread).
-__device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool cut_by_count, unsigned int k, float p,
+__device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool cut_by_count, unsigned int k, float p, float least,
                                     bool mass_of_row, unsigned long long row_mass, float u, float* s_list /* [kSampleThreads] */,
                                     unsigned long long* s_wave /* [16] */, float* s_piece /* [16] */, int* s_pick /* [2] */) {
     __shared__ __attribute__((aligned(16))) unsigned long long s_fixed[kSampleThreads];
@@ -781,6 +808,7 @@ __device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool 
         if (need == 0ull) need = 1ull;
         keep = keep && mass_above < need;
     }
+    keep = keep && wj >= least;
     // inverse CDF in index order: prefix sums inside the wavefronts, then over them
     const float mine = keep ? wj : 0.f;
     float incl = mine;
@@ -885,7 +913,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     const float* __restrict__ top_p, const float* __restrict__ uniform, int32_t* __restrict__ out,
     float* __restrict__ weights, int vocab, const int32_t* __restrict__ cand_idx, const int32_t* __restrict__ cand_count,
     const int32_t* __restrict__ listed, const int32_t* __restrict__ list_count, const int32_t* __restrict__ best_in, const unsigned long long* __restrict__ row_mass,
-    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin) {
+    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin,
+    const float* __restrict__ min_p) {
     __shared__ float s_val[16];
     __shared__ int s_idx[16];
     __shared__ unsigned int hist[256];
@@ -905,7 +934,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     float* w = weights + static_cast<size_t>(r) * vocab;
     const int32_t* idx_of = cand_idx ? cand_idx + static_cast<size_t>(r) * vocab : nullptr;
     // (a row's few numbers at once: behind the branches that ask for them each would be a wait of its own)
-    const float temp = temperature[r], p = top_p[r], u = uniform[r];
+    const float temp = temperature[r], p = top_p[r], u = uniform[r], least = least_of(min_p, r);
     const int k = top_k[r];
     int known_best = 0, is_listed = 0, direct = -1, count = 0, more = 0;
     if (cand_idx) {
@@ -970,7 +999,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
             const float wj = j < n ? s_list[j] : 0.f;
             const int ij = j < n ? s_order[j] : 0x7fffffff;
             __syncthreads();
-            vocab = order_candidates(wj, ij, n, static_cast<unsigned int>(k), s_list, s_order, hist);
+            // (a list by min_p: all of it)
+            vocab = order_candidates(wj, ij, n, k > 0 && k < full_vocab ? static_cast<unsigned int>(k) : 0xffffffffu, s_list, s_order, hist);
         } else {
             // more than a thousand equals: the thresholds from the list, brought together in the first piece's place and behind it
             // (every piece's part moves towards the front, one piece after the other), the draw from the row
@@ -998,7 +1028,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     const unsigned long long mass = cand_idx && !k_active ? row_mass[r] : 0ull;
     if (vocab <= kSampleThreads) {                   // a short row or list: one thread per token
         const float wj = unordered ? s_list[threadIdx.x] : static_cast<int>(threadIdx.x) < vocab ? w[threadIdx.x] : 0.f;
-        const int at = pick_from_short_list(wj, vocab, k_active && k < vocab, static_cast<unsigned int>(k), p,
+        const int at = pick_from_short_list(wj, vocab, k_active && k < vocab, static_cast<unsigned int>(k), p, least,
                                             cand_idx && !k_active, mass, u, s_list, s_wave, s_piece, s_pick);
         if (threadIdx.x == 0) out[r] = at < 0 ? best : unordered ? s_order[at] : idx_of ? idx_of[at] : at;
         return;
@@ -1032,8 +1062,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
             top = bin == 0 ? 0x3f800001u : static_cast<uint32_t>(128 - min(bin, kTopBins)) << 23;
             above = direct_target[r];
         }
-        threshold = select_by_mass(w, vocab, threshold, top, above, need, s_wave, &s_a, &s_b, &s_above);
+        if (above == kAllPass) threshold = 0u;
+        else threshold = select_by_mass(w, vocab, threshold, top, above, need, s_wave, &s_a, &s_b, &s_above);
     }
+    threshold = max(threshold, __float_as_uint(least));
     // inverse CDF in index order.  Every wavefront owns a contiguous piece of the row; the piece that holds the
     // drawn point is then walked 64 tokens at a time with a prefix sum over the lanes.
     if (unordered) vocab = full_vocab;
@@ -1159,12 +1191,12 @@ extern "C" int egpt_argmax_static(const float* logits, int32_t* out, int n_rows,
 
 // weights: scratch for n_rows * vocab floats.
 extern "C" int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                           const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream) {
+                           const float* min_p, const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !weights || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
     sample_kernel<<<n_rows, kSampleThreads, 0, static_cast<hipStream_t>(stream)>>>(
-        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, min_p);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }
@@ -1185,7 +1217,7 @@ extern "C" size_t egpt_sample_workspace(int n_rows, int vocab) {
 }
 
 extern "C" int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                                const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream) {
+                                const float* min_p, const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !workspace || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
@@ -1211,14 +1243,15 @@ extern "C" int egpt_sample_wide(const float* logits, const float* temperature, c
     argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, sub, vocab);
     EGPT_CHECK_LAUNCH();
     sample_count_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, pv, pi, sub, best, listed, list_count, cand_w, cand_idx,
-                                                                    piece_count, piece_mass, vocab);
+                                                                    piece_count, piece_mass, vocab, top_p, min_p);
     EGPT_CHECK_LAUNCH();
     sample_compact_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, top_p, uniform, best, piece_count,
                                                                       piece_mass, listed, cand_w, cand_idx, cand_count, row_mass,
-                                                                      direct_piece, direct_target, last_bin, vocab);
+                                                                      direct_piece, direct_target, last_bin, vocab, min_p);
     EGPT_CHECK_LAUNCH();
     sample_kernel<<<n_rows, kSampleThreads, 0, s>>>(logits, temperature, top_k, top_p, uniform, out, cand_w, vocab, cand_idx,
-                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin);
+                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin,
+                                                    min_p);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }

@@ -32,7 +32,29 @@ Methods of a backend (T tokens, B requests, R rows, act = bfloat16 or float32):
   swiglu(gate_up act[T,2I], out act[T,I], activation='silu')   out = f(gate_up[:, :I]) * gate_up[:, I:], f silu or 'gelu_tanh', the
         tanh form of gelu (product_swiglu and gate_up_swiglu take the same)
   argmax(logits f32[R,V], out i32[R])            lowest index among equal maxima
-  sample(logits f32[R,V], temperature f32[R], top_k i32[R], top_p f32[R], uniform f32[R], out i32[R])
+  sample(logits f32[R,V], temperature f32[R], top_k i32[R], top_p f32[R], uniform f32[R], out i32[R], min_p=None)
+        the weights exp((x - max) / temperature), cut to the top_k greatest (0 or V: all; ties whole), then to the fewest greatest
+        whose mass reaches top_p (1: all; ties whole), then, with min_p f32[R] (0: all), to those of at least min_p times the
+        greatest; the first token in index order whose running sum of what is left exceeds uniform * that sum; the lowest index of the
+        greatest where the temperature is 0 or less
+
+  tree_attention(qkv, out act[T,nq*hd], k_cache, v_cache, block_table i32[B,W], q_start i32[B], q_len i32[B], kv_len i32[B],
+                 visible i64[T], nq, nkv, hd, page_size, scale, max_q_len, max_kv_len, window=0, positions=None)
+        attention for trees of drafted tokens (operands as paged_attention; queries are the first nq * hd columns of qkv): request
+        b's q_len[b] <= 64 nodes are the last ones of its kv_len[b] tokens in the cache, in any order of their own.  A node reads the
+        tokens before the tree (with a window those at places > positions[t] - window, positions i32[T]) and the nodes m whose
+        bit m of `visible` is set (`draft_masks` makes them of parents); a row that sees nothing is zeros.  q_start ascends; rows of
+        qkv that no request has keep their `out`
+  accept_drafts(tokens i32[T], parents i32[T], sampled i32[T], q_start i32[B], q_len i32[B]) -> path i32[B,64], count i32[B],
+                accepted i32[B,64]
+        the walk through a tree whose node 0 is the token sampled last and whose node i > 0 drafts tokens[i] behind node
+        parents[i] < i: from the root to the child whose token is what the model sampled behind its parent (the lowest of several) until there is
+        none.  path: the nodes passed, the root among them, count of them; accepted: what was sampled behind each, the request's
+        new tokens; -1 behind the last
+  keep_drafts(k_cache [slabs,P,nkv,page_size,dk] | [P,...], v_cache [slabs,P,nkv,dv,page_size] | [P,...], block_table i32[B,W],
+              start i32[B], path i32[B,L], count i32[B])
+        key and value of the first count[b] nodes of an ascending path, which lie at places start[b] + path[b,k] of their request, go to places
+        start[b] + k, in all slabs (in place; the other nodes' places hold what they held)
 
   (head_norm_store, latent_prep and sigmoid_gate also take row_ss f32[S2,T], hidden, norm_eps: the product, float32
    partial sums, then still lacks each row's factor 1/sqrt(sum_s row_ss[s] / hidden + norm_eps), as `product_normed`
@@ -164,6 +186,7 @@ class KernelBackend:
     fuses nothing.  `kernels.hip.HipKernels` overrides them where its kernels cover the shapes."""
 
     name = "abstract"
+    max_tree_nodes = 64     # drafted tokens of one request that one step checks at most, the root among them
     max_head_dim = 256      # the widest attention head the kernels take: a part refuses more when it is built
     fused_rows = 0          # products whose x operand is computed while it is staged take at most this many rows
     max_window_attention_dim = 1024     # the widest key or value that window_attention takes
@@ -300,6 +323,22 @@ class KernelBackend:
     def rope_table(self, positions, inv_freq):
         """float32 [T, half, 2]: (cos, sin) of every token's angles, for the kernels that rotate; or None."""
         return None
+
+
+def draft_masks(parents, window: int = 0) -> tuple[list[int], list[int]]:
+    """Of one request's tree of drafted tokens, parents[0] = -1 and parents[i] < i: every node's depth, and the bits of the nodes
+    that it sees, its ancestors (with a window those fewer than `window` steps above it) and itself, as a signed 64-bit number."""
+    if len(parents) > KernelBackend.max_tree_nodes:
+        raise ValueError(f"a request's tree has at most {KernelBackend.max_tree_nodes} nodes, not {len(parents)}")
+    depth: list[int] = []
+    path: list[list[int]] = []
+    for i, p in enumerate(parents):
+        if (p != -1) if i == 0 else not 0 <= p < i:
+            raise ValueError(f"node {i} of a tree of drafted tokens has parent {p}: node 0 has none (-1), another's lies before it")
+        depth.append(depth[p] + 1 if i else 0)
+        path.append((path[p] if i else []) + [i])
+    masks = [sum(1 << m for m in (q[-window:] if window else q)) for q in path]
+    return depth, [m - (1 << 64) if m >> 63 else m for m in masks]
 
 
 class KernelsUnavailable(RuntimeError):

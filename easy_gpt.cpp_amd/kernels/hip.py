@@ -31,7 +31,7 @@ def _load_library() -> ctypes.CDLL:
         lib = ctypes.CDLL(path)
     except (build.BuildError, OSError) as e:
         raise KernelsUnavailable(f"the HIP kernel library could not be built or loaded: {e}") from e
-    if lib.egpt_abi_version() != 29:
+    if lib.egpt_abi_version() != 30:
         raise KernelsUnavailable(f"{path} has an unexpected ABI version")
     return lib
 
@@ -109,8 +109,11 @@ class HipKernels(KernelBackend):
             "egpt_attention_any_tiled": [vp, vp, vp, vp, vp, i, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_attention_any_decode": [vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i, i, i, i, i, f, i, i, i, vp],
             "egpt_argmax": [vp, vp, vp, i, i, vp],
-            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
-            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_tree_attention_generic": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
+            "egpt_accept_drafts": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp],
+            "egpt_keep_drafts": [vp, vp, vp, i, vp, vp, i, vp, i, i, i, i, i, i, i, i, vp],
             "egpt_gemm_gate_up_swiglu": [vp, vp, vp, i, i, i, i, i, vp],
             "egpt_embed_rmsnorm": [vp, vp, vp, f, vp, i, i, i, i, i, vp],
             "egpt_head_norm_store": [vp, i, vp, i, i, f, i, vp, vp, vp, f, i, vp, i, f, vp, vp, vp, i, i, i, i, i, i, vp, vp, f, i, i, vp, i,
@@ -2172,7 +2175,7 @@ class HipKernels(KernelBackend):
         scratch = torch.empty(r * 64, dtype=_F32, device=logits.device) if v >= 8192 else None
         self._run("egpt_argmax", logits.data_ptr(), out.data_ptr(), self._ptr(scratch), r, v, self._stream())
 
-    def sample(self, logits, temperature, top_k, top_p, uniform, out):
+    def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None):
         r, v = logits.shape
         self._need(logits, "logits", _F32)
         self._need(temperature, "temperature", _F32, (r,))
@@ -2180,12 +2183,97 @@ class HipKernels(KernelBackend):
         self._need(top_p, "top_p", _F32, (r,))
         self._need(uniform, "uniform", _F32, (r,))
         self._need(out, "out", _I32, (r,))
+        if min_p is not None:
+            self._need(min_p, "min_p", _F32, (r,))
         if v >= 8192:
             # a wide vocabulary: the row-wide passes by many workgroups, the selection on the tokens that are left
             space = torch.empty(int(self.lib.egpt_sample_workspace(r, v)), dtype=torch.uint8, device=logits.device)
-            self._run("egpt_sample_wide", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+            self._run("egpt_sample_wide", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), self._ptr(min_p),
                       uniform.data_ptr(), out.data_ptr(), space.data_ptr(), r, v, self._stream())
             return
         weights = torch.empty((r, v), dtype=_F32, device=logits.device)
-        self._run("egpt_sample", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+        self._run("egpt_sample", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), self._ptr(min_p),
                   uniform.data_ptr(), out.data_ptr(), weights.data_ptr(), r, v, self._stream())
+
+    # ------------------------------------------------------------------ drafted tokens
+    @staticmethod
+    def _here(t: torch.Tensor, *others) -> None:
+        """These operators launch on the current device's stream, so that is where their operands have to be."""
+        device = t.device
+        for o in others:
+            if o is not None and o.device != device:
+                raise ValueError(f"operands lie on {device} and on {o.device}")
+        if device.index != torch.cuda.current_device():
+            raise ValueError(f"operands lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+    def tree_attention(self, qkv, out, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, nq, nkv, hd, page_size, scale,
+                       max_q_len, max_kv_len, window=0, positions=None):
+        t = qkv.shape[0]
+        if nkv < 1 or nq < 1 or nq % nkv:
+            raise ValueError(f"the number of query heads ({nq}) must be a multiple of that of key heads ({nkv})")
+        if not 1 <= hd <= self.max_head_dim:
+            raise ValueError(f"head size {hd} is not supported by the attention kernels (1 to {self.max_head_dim})")
+        if max_q_len > self.max_tree_nodes:
+            raise ValueError(f"a request's tree has at most {self.max_tree_nodes} nodes, not {max_q_len}")
+        if window < 0:
+            raise ValueError("the window must be >= 0")
+        dt = self._act(qkv, "qkv")
+        self._need(qkv, "qkv", None, (t, (nq + 2 * nkv) * hd))
+        self._need(out, "out", qkv.dtype, (t, nq * hd))
+        self._caches(k_cache, v_cache, qkv.dtype, nkv, page_size, hd)
+        self._need(block_table, "block_table", _I32)
+        if block_table.dim() != 2:
+            raise ValueError(f"block_table must be [requests, pages of the longest], got {tuple(block_table.shape)}")
+        b, width = block_table.shape
+        for name, v in (("q_start", q_start), ("q_len", q_len), ("kv_len", kv_len)):
+            self._need(v, name, _I32, (b,))
+        self._need(visible, "visible", _I64, (t,))
+        if window:
+            if positions is None:
+                raise ValueError("a window needs the nodes' positions")
+            self._need(positions, "positions", _I32, (t,))
+        if max_kv_len > width * page_size:
+            raise ValueError(f"block table of width {width} cannot hold {max_kv_len} tokens at page size {page_size}")
+        self._here(qkv, out, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, positions if window else None)
+        if t == 0 or b == 0:
+            return
+        self._run("egpt_tree_attention_generic", qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                  width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
+                  positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), dt, self._stream())
+
+    def accept_drafts(self, tokens, parents, sampled, q_start, q_len):
+        t, b = tokens.shape[0], q_len.shape[0]
+        for name, v, n in (("tokens", tokens, t), ("parents", parents, t), ("sampled", sampled, t), ("q_start", q_start, b), ("q_len", q_len, b)):
+            self._need(v, name, _I32, (n,))
+        self._here(tokens, parents, sampled, q_start, q_len)
+        path, accepted = torch.empty((2, b, self.max_tree_nodes), dtype=_I32, device=tokens.device)
+        count = torch.empty(b, dtype=_I32, device=tokens.device)
+        self._run("egpt_accept_drafts", tokens.data_ptr(), parents.data_ptr(), sampled.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), b, t,
+                  path.data_ptr(), count.data_ptr(), accepted.data_ptr(), self._stream())
+        return path, count, accepted
+
+    def keep_drafts(self, k_cache, v_cache, block_table, start, path, count):
+        dt = self._act(k_cache, "k_cache")
+        self._need(k_cache, "k_cache")
+        self._need(v_cache, "v_cache", k_cache.dtype)
+        if k_cache.dim() not in (4, 5) or v_cache.dim() != k_cache.dim():
+            raise ValueError("k_cache and v_cache must be [pages, ...] or [slabs, pages, ...] of pages of keys and of values")
+        pages, nkv, page_size, dk = k_cache.shape[-4:]
+        dv = v_cache.shape[-2]
+        if tuple(v_cache.shape) != (*k_cache.shape[:-2], dv, page_size):
+            raise ValueError(f"v_cache must be {(*k_cache.shape[:-2], dv, page_size)} beside keys {tuple(k_cache.shape)}, got {tuple(v_cache.shape)}")
+        self._need(block_table, "block_table", _I32)
+        self._need(path, "path", _I32)
+        if block_table.dim() != 2 or path.dim() != 2:
+            raise ValueError("block_table and path must be [requests, ...]")
+        b, width = block_table.shape
+        if path.shape[0] != b:
+            raise ValueError(f"path must have {b} rows, got {path.shape[0]}")
+        self._need(start, "start", _I32, (b,))
+        self._need(count, "count", _I32, (b,))
+        self._here(k_cache, v_cache, block_table, start, path, count)
+        if k_cache.numel() == 0 or b == 0 or width == 0 or path.shape[1] == 0:
+            return
+        self._run("egpt_keep_drafts", k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), width, start.data_ptr(), path.data_ptr(),
+                  path.shape[1], count.data_ptr(), b, k_cache.shape[0] if k_cache.dim() == 5 else 1, pages, page_size, nkv, dk, dv, dt,
+                  self._stream())
