@@ -409,6 +409,14 @@ int egpt_tree_attention_generic(const void* qkv, void* out, const void* k_cache,
                                 int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
                                 const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,
                                 int dtype, void* stream);
+// The same on the matrix cores: keys of whole 16 bytes, page sizes that are multiples of 16, operands on 16 bytes.  No request brings more than max_q_len
+// <= 64 nodes.  A request's keys are cut into parts of `chunk`, a multiple of 128 up to 8,192, at most `parts` of them; with more than one, part_o
+// [parts][n_tokens][nq][hd] and part_ml [parts][n_tokens][nq][2] (float32) hold their results until a second kernel joins them.  shape: blocks
+// of 32 rows that a workgroup takes, 1, 4 and, up to head size 128 (float32: 64), 2, and in bfloat16 8.
+int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                        int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
+                        const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,
+                        int max_q_len, int shape, int parts, int chunk, int dtype, void* stream);
 // path, accepted int32 [n_seqs][64], count int32 [n_seqs]
 int egpt_accept_drafts(const int32_t* tokens, const int32_t* parents, const int32_t* sampled, const int32_t* q_start, const int32_t* q_len, int n_seqs,
                        int n_tokens, int32_t* path, int32_t* count, int32_t* accepted, void* stream);

@@ -6,8 +6,11 @@
 //     j = kv - n + m   and bit m of visible_i is set                 (node m; a request has at most 64)
 // and is softmax_j(scale q . k_j) v_j over those, zeros where there are none.  A number that a row does not see does not reach it, be it an
 // infinity or a NaN.
+#include <type_traits>
+
 #include "api.h"
 #include "common.h"
+#include "lds_loads.h"
 
 namespace egpt {
 
@@ -123,6 +126,490 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
     }
 }
 
+
+// ---- on the matrix cores: bfloat16 and float32, keys and values of whole 16 bytes, pages of multiples of 16 tokens
+//
+// Rows of one request and kv head, (node, head) pairs node-major, in blocks of 32, a block to a wavefront; RB wavefronts share a tile of KT keys, and KS such groups
+// take every KS-th tile.  The scores come transposed, S^T[key, row] = K Q^T on 32 x 32 products, so that a lane has 16 of a block's 32 scores of ONE row (the lane 32
+// further has the others): the softmax is arithmetic within a lane but for one exchange, and the probabilities lie as the second product, O^T += V^T P^T,
+// takes them, without a trip through LDS.  An operand is 16 bytes a lane in either type: one product of bfloat16, 8 x 2 features of a row, four of
+// float32, 4 x 2; the order of the summed index is free as long as both sides have the same, so bfloat16 reads the keys of a block with bits 2 and 3 of
+// their number exchanged, which gives a lane eight neighbouring keys for the second product, as a page has a feature's values.
+//
+// Tiles go from memory straight to LDS, NS - 1 of them ahead of their use, one barrier a tile.  A load takes 1,024 bytes that lie in one page: a
+// resource with that page's base, bounded by it, and a constant offset per lane.  Keys lie in rows, 16-byte pieces exchanged by the row's number, values as a page of 16
+// tokens has them: either way 64 lanes read different banks.  A head that is no power of two is filled up with zeros by the loads' bounds.
+//
+// A request's keys are cut into parts of `chunk`, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
+// parts leave the unnormalised result with its maximum and sum, and tree_combine_kernel joins them.
+typedef __attribute__((ext_vector_type(8))) __bf16 tree_bf16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float tree_f32x4;
+
+template <typename T>
+__device__ __forceinline__ f32x16 product_of(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(tree_bf16x8, a), __builtin_bit_cast(tree_bf16x8, b), c, 0, 0, 0);
+    } else {
+        const tree_f32x4 x = __builtin_bit_cast(tree_f32x4, a), y = __builtin_bit_cast(tree_f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// Two bfloat16 numbers or a float32 as bits, by integer arithmetic (comparisons of every element leave the scalar registers no room): at the top bit of
+// each number whether it is an infinity or a NaN, and whether it is a NaN.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(unsigned x) {
+    if constexpr (sizeof(T) == 2) return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    else return ((x & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+}
+template <typename T>
+__device__ __forceinline__ unsigned fraction_of(unsigned x) {
+    if constexpr (sizeof(T) == 2) return (((x & 0x007f007fu) + 0x007f007fu) & 0x00800080u) << 8;
+    else return ((x & 0x007fffffu) + 0x007fffffu) << 8 & 0x80000000u;
+}
+// All ones in the numbers whose top bit is set, and the number 1 there.
+template <typename T>
+__device__ __forceinline__ unsigned filled(unsigned top) {
+    if constexpr (sizeof(T) == 2) return (top >> 15) * 0xffffu;
+    else return static_cast<unsigned>(static_cast<int>(top) >> 31);
+}
+template <typename T>
+__device__ __forceinline__ unsigned one_where(unsigned top) { return filled<T>(top) & (sizeof(T) == 2 ? 0x3f803f80u : 0x3f800000u); }
+// All ones if bit `at` of x is set.
+__device__ __forceinline__ unsigned bit_filled(unsigned x, int at) { return static_cast<unsigned>(static_cast<int>(x << (31 - at)) >> 31); }
+
+constexpr int kGroup = 16;                       // keys that a load's base is found for: never more than a page's
+constexpr int kMostGroups = 512;                 // of a workgroup's part
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"        // (m0 is a reserved register; nothing else here uses it)
+// 16 bytes a lane from byte `offset` of a resource to LDS, at address `to` (the same for the whole wavefront) + 16 x lane; zeros past its end.
+__device__ __forceinline__ void load_1k(r_i32x4 resource, int offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(resource)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+struct TreeSizes {
+    int table_width, n_pages, page_size, nq, nkv, hd, group, n_seqs, parts, chunk, blocks, window, n_tokens;
+    unsigned magic_parts, magic_nkv, magic_blocks, magic_group, magic_page, magic_chunk;
+    float scale;
+};
+
+template <typename T, int HD, int RB, int KS, int KT, int NS>
+constexpr int tree_lds() {
+    constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = (KS - 1) * RB * 64 * (HD / 2 + 2) * 4;
+    return (stages > join ? stages : join) + kMostGroups * 8 + 16;
+}
+
+template <typename T, int HD, int RB, int KS, int KT, int NS>
+__global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1) void tree_attention_kernel(
+    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start, const int32_t* __restrict__ block_table,
+    const T* __restrict__ qkv, const long long* __restrict__ visible, const int32_t* __restrict__ positions, const T* __restrict__ k_cache,
+    const T* __restrict__ v_cache, T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml, TreeSizes z) {
+    constexpr int SZ = sizeof(T);
+    constexpr int ROWB = HD * SZ, PIECES = ROWB / 16, KC = ROWB / 32, DB = HD / 32, KB = KT / 32;
+    constexpr int HALF = KT * ROWB, TILE = 2 * HALF;             // bytes of a tile's keys, and of it all
+    constexpr int LOADS = HALF / 1024 / RB;                      // of a wavefront and tile, keys and values each
+    constexpr int PER_GROUP = ROWB / 64;                         // loads of a group of 16 keys
+    constexpr int OWN = LOADS > PER_GROUP ? LOADS / PER_GROUP : 1, EACH = LOADS > PER_GROUP ? PER_GROUP : LOADS;
+    constexpr int STEPS = SZ == 2 ? 2 : 4;                       // second products of a block of 32 keys: 32 bytes of a feature each
+    static_assert(LOADS >= 1 && HALF % (1024 * RB) == 0 && OWN * EACH == LOADS, "every wavefront loads as much");
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int SPACE = tree_lds<T, HD, RB, KS, KT, NS>() - kMostGroups * 8 - 16;
+    int2* const s_place = reinterpret_cast<int2*>(smem + SPACE);          // page and offset of every group of the part
+    int* const s_missing = reinterpret_cast<int*>(smem + SPACE + kMostGroups * 8);
+    const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 32, lh = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), rb = wave % RB, ksi = wave / RB;
+
+    // Which part of which request and kv head, and which block of its rows.  Workgroups go to the eight dies in turn: the blocks of rows that read the same
+    // keys follow each other on one of them.
+    const int slot = blockIdx.x / 8;
+    const int unit0 = divided(slot, z.blocks, z.magic_blocks);
+    const int block = slot - unit0 * z.blocks, unit = unit0 * 8 + blockIdx.x % 8;
+    const int pair = divided(unit, z.parts, z.magic_parts), part = unit - pair * z.parts;
+    const int b = divided(pair, z.nkv, z.magic_nkv), kvh = pair - b * z.nkv;
+    if (b >= z.n_seqs) return;
+    const int n = q_len[b], rows = n * z.group, row0 = block * 32 * RB;
+    if (row0 >= rows) return;
+    const int kv_all = kv_len[b], before = kv_all - n, kv = min(kv_all, z.table_width * z.page_size);
+    const int qs = q_start[b];
+    const int n_parts = min(divided(max(kv_all, 1) - 1, z.chunk, z.magic_chunk) + 1, z.parts);
+    if (part >= n_parts) return;
+
+    // this lane's row
+    const int r = row0 + rb * 32 + lr;
+    const bool valid = r < rows && qs >= 0 && qs + divided(r, z.group, z.magic_group) < z.n_tokens;
+    const int node = valid ? divided(r, z.group, z.magic_group) : 0;
+    const int head = kvh * z.group + (valid ? r - node * z.group : 0);
+    const int token = qs + node;
+    unsigned long long bits = valid ? static_cast<unsigned long long>(visible[token]) : 0ull;
+    int lo = valid && z.window > 0 ? min(max(0, positions[token] - z.window + 1), max(before, 0)) : 0;
+    if (!valid) lo = 0x7fffffff;
+    const int key_bytes = z.hd * SZ;
+    u32x4 q[KC];
+    {
+        const char* qp = reinterpret_cast<const char*>(qkv + static_cast<size_t>(token) * (z.nq + 2 * z.nkv) * z.hd + head * z.hd);
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            const int at = i * 32 + lh * 16;
+            q[i] = valid && at < key_bytes ? *reinterpret_cast<const u32x4*>(qp + at) : u32x4{0u, 0u, 0u, 0u};
+            if (z.scale < 0.f) q[i] ^= SZ == 2 ? 0x80008000u : 0x80000000u;        // (the greatest score is the greatest product then as well)
+        }
+    }
+    // the keys of this part that the workgroup's rows see: from the lowest window's first on
+    int lo_wave_least = 0, lo_wave_most = 0;
+    if (z.window > 0) {
+        float least = valid ? static_cast<float>(lo) : 3.0e38f, most = valid ? static_cast<float>(lo) : 0.f;      // (places are below 2^24, or the bounds a little wider)
+        least = -wave_max(-least);
+        most = wave_max(most);
+        lo_wave_least = least > 2.0e9f ? 0 : max(0, static_cast<int>(least) - (least > 16777216.f ? 256 : 0));
+        lo_wave_most = static_cast<int>(fminf(most, 2.0e9f)) + (most > 16777216.f ? 256 : 0);
+    }
+    const int from = part * z.chunk, to = min(kv, from + z.chunk);
+    const int groups = to > from ? (to - from + kGroup - 1) / kGroup : 0;
+    {
+        if (tid == 0) *s_missing = 0;
+        __syncthreads();
+        const int32_t* table = block_table + static_cast<size_t>(b) * z.table_width;
+        for (int i = tid; i < groups; i += 64 * RB * KS) {
+            const int key = from + i * kGroup, at = divided(key, z.page_size, z.magic_page);
+            int page = table[at];
+            if (page < 0 || page >= z.n_pages) {
+                page = -1;
+                *s_missing = 1;                                  // (some rows' tiles may lie before their window, where pages have been given back)
+            }
+            s_place[i] = int2{page, key - at * z.page_size};
+        }
+        __syncthreads();
+    }
+    const bool missing = *s_missing != 0;
+
+    const size_t head_bytes = static_cast<size_t>(z.page_size) * key_bytes, page_bytes = head_bytes * z.nkv;
+    const char* const k_head = reinterpret_cast<const char*>(k_cache) + kvh * head_bytes;
+    const char* const v_head = reinterpret_cast<const char*>(v_cache) + kvh * head_bytes;
+    const int row_swap = PIECES >= 16 ? 15 : 7;
+    const int first_load = rb * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
+    int k_at[EACH], v_at[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int u = load_first + j;
+        const int key = u * (1024 / ROWB) + lane / PIECES;                   // of the group's 16
+        const int order = SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key;       // bits 2 and 3 exchanged
+        const int piece = (lane % PIECES) ^ (order & row_swap);
+        k_at[j] = piece * 16 < key_bytes ? key * key_bytes + piece * 16 : kNowhere;
+        const int d = u * (64 / SZ) + lane / SZ;
+        const int v_piece = SZ == 2 ? lane % 2 : (lane % 4) ^ (d >> 2 & 3);
+        v_at[j] = d < z.hd ? d * z.page_size * SZ + v_piece * 16 : kNowhere;
+    }
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)smem));
+    const int n_tiles = (groups * kGroup + KT - 1) / KT, rounds = (n_tiles + KS - 1) / KS;
+    auto load_tile = [&](int round) {
+        const unsigned base = lds0 + (round % NS * KS + ksi) * TILE + first_load * 1024;
+        const int g0 = (round * KS + ksi) * (KT / kGroup) + group_first;
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int2 place = g0 + o < groups ? s_place[g0 + o] : int2{-1, 0};
+            const int page = __builtin_amdgcn_readfirstlane(place.x), off = __builtin_amdgcn_readfirstlane(place.y);
+            const size_t at = static_cast<size_t>(max(page, 0)) * page_bytes;
+            const r_i32x4 keys = buffer_of(k_head + at + static_cast<size_t>(off) * key_bytes, page < 0 ? 0 : kGroup * key_bytes);
+            const r_i32x4 values = buffer_of(v_head + at + static_cast<size_t>(off) * SZ, page < 0 ? 0 : head_bytes - static_cast<size_t>(off) * SZ);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) load_1k(keys, k_at[j], base + (o * PER_GROUP + j) * 1024);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) load_1k(values, v_at[j], base + HALF + (o * PER_GROUP + j) * 1024);
+        }
+    };
+
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    const float scale2 = fabsf(z.scale) * 1.4426950408889634f;          // exponentials are taken to the base 2
+    const int my_key = SZ == 2 ? (lr & 3) | (lr >> 1 & 4) | (lr << 1 & 8) | (lr & 16) : lr;
+    const int k_row = my_key * ROWB, k_piece = (lh ^ (lr & row_swap)) * 16;
+    const int v_row = lr * kGroup * SZ + (SZ == 2 ? lh * 16 : ((lh ^ (lr >> 2 & 3)) * 16));
+
+    auto piece_at = [&](const char* at) { return *reinterpret_cast<const u32x4*>(at); };
+    auto values_at = [&](const char* tile, int kb, int step, int d) {
+        const int g = kb * 2 + (SZ == 2 ? step : step / 2);
+        const int row = SZ == 2 ? v_row : v_row ^ ((step % 2) * 32);
+        return piece_at(tile + HALF + (g * HD + d * 32) * kGroup * SZ + row);
+    };
+    // A tile.  MASKED: its scores are compared with what the row sees, and its values may hold numbers that are none, which rows that do not see them are kept from.
+    auto tile_of = [&](auto masked, const char* tile, int key0, int group0) {
+        constexpr bool MASKED = decltype(masked)::value;
+        constexpr int R = SZ == 2 ? 8 : 4;                                      // neighbouring keys of a lane
+        f32x16 s[KB];
+        unsigned sees[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KC; ++i) s[kb] = product_of<T>(piece_at(tile + kb * 32 * ROWB + k_row + (k_piece ^ (i * 32))), q[i], s[kb]);
+            if constexpr (MASKED) {
+                const int k0 = key0 + kb * 32, cut = before - k0;               // keys of the block before the tree
+                unsigned long long w = cut >= 0 ? (cut < 32 ? bits << cut : 0ull) : (cut > -64 ? bits >> -cut : 0ull);
+                unsigned early = cut >= 32 ? 0xffffffffu : cut > 0 ? (1u << cut) - 1u : 0u;
+                const int skip = lo - k0;
+                if (skip > 0) early = skip >= 32 ? 0u : early & (0xffffffffu << skip);
+                unsigned all = static_cast<unsigned>(w) | early;
+                const int end = kv - k0;
+                if (end < 32) all = end > 0 ? all & ((1u << end) - 1u) : 0u;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    if (group0 + kb * 2 + g >= groups || s_place[group0 + kb * 2 + g].x < 0) all &= g == 0 ? 0xffff0000u : 0x0000ffffu;
+                if (!valid) all = 0u;
+                sees[kb] = all >> (lh * R);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const unsigned it = bit_filled(sees[kb], e / R * 2 * R + e % R);
+                    s[kb][e] = __uint_as_float((__float_as_uint(s[kb][e]) & it) | (0xff800000u & ~it));
+                }
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+        mx = fold_32_apart(mx, MaxOf());
+        if (__any(mx > m_run)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale2);
+            l_run *= alpha;
+            m_run = m_new;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
+        }
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;
+        [[maybe_unused]] const float m_scaled = m_use * scale2;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                // (bfloat16: the argument by one operation, whose error, 2^-24 of the maximum, is nothing beside the probabilities' rounding)
+                float p = SZ == 2 ? __builtin_amdgcn_exp2f(fmaf(s[kb][e], scale2, -m_scaled)) : __builtin_amdgcn_exp2f((s[kb][e] - m_use) * scale2);
+                if constexpr (MASKED) p = __uint_as_float(__float_as_uint(p) & bit_filled(sees[kb], e / R * 2 * R + e % R));
+                s[kb][e] = p;
+                sum += p;
+            }
+            l_run += sum;
+            [[maybe_unused]] unsigned strange = 0u;
+#pragma unroll
+            for (int step = 0; step < STEPS; ++step) {
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (SZ == 2) p[e] = bf16_pair(s[kb][step * 8 + 2 * e], s[kb][step * 8 + 2 * e + 1]);
+                    else p[e] = __float_as_uint(s[kb][step * 4 + e]);
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    u32x4 v = values_at(tile, kb, step, d);
+                    if constexpr (MASKED) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned it = not_finite<T>(v[e]);
+                            strange |= it;
+                            v[e] &= ~filled<T>(it);
+                        }
+                    }
+                    acc[d] = product_of<T>(v, p, acc[d]);
+                }
+            }
+            if constexpr (MASKED) {
+                // Values that are no finite numbers, left out above: how many infinities of either sign (a NaN is both) each row sees, by the same products of ones,
+                // and what they make of the sum.
+                if (__any(strange != 0u)) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        f32x16 up, down;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) up[e] = down[e] = 0.f;
+#pragma unroll
+                        for (int step = 0; step < STEPS; ++step) {
+                            const u32x4 v = values_at(tile, kb, step, d);
+                            u32x4 seen, above, below;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const unsigned it = not_finite<T>(v[e]), nan = fraction_of<T>(v[e]);
+                                above[e] = one_where<T>(it & (nan | ~v[e]));
+                                below[e] = one_where<T>(it & (nan | v[e]));
+                                if constexpr (SZ == 2)
+                                    seen[e] = (bit_filled(sees[kb], step * 16 + 2 * e) & 0x3f80u) | (bit_filled(sees[kb], step * 16 + 2 * e + 1) & 0x3f800000u);
+                                else seen[e] = bit_filled(sees[kb], step * 8 + e) & 0x3f800000u;
+                            }
+                            up = product_of<T>(above, seen, up);
+                            down = product_of<T>(below, seen, down);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[d][e] += up[e] * 3.0e38f * 3.0e38f - down[e] * 3.0e38f * 3.0e38f;      // (0 or an infinity each)
+                    }
+                }
+            }
+        }
+    };
+
+    // (tiles before every row's window are not loaded)
+    const int lo_block = z.window > 0 ? max(0, lo_wave_least) : 0;
+    int first_round = 0;
+    if (z.window > 0) {
+        __shared__ int s_least[8];
+        if (lane == 0) s_least[wave] = row0 + rb * 32 < rows ? lo_block : 0x7fffffff;
+        __syncthreads();
+        int least = 0x7fffffff;
+        for (int w = 0; w < RB * KS; ++w) least = min(least, s_least[w]);
+        first_round = max(0, min(least, before) - from) / (KT * KS);
+    }
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+        if (first_round + i < rounds) load_tile(first_round + i);
+    for (int round = first_round; round < rounds; ++round) {
+        // this wavefront's loads of the tile are there when no more than those of the later ones are on their way; then everybody's
+        if (round + NS - 1 <= rounds) arrived<(NS - 2) * 2 * LOADS>();
+        else arrived<0>();
+        __syncthreads();
+        if (round + NS - 1 < rounds) load_tile(round + NS - 1);
+        const int tile = round * KS + ksi, key0 = from + tile * KT;
+        if (tile >= n_tiles) continue;
+        const char* const at = smem + (round % NS * KS + ksi) * TILE;
+        if (!missing && key0 + KT <= min(before, kv) && key0 >= lo_wave_most) tile_of(std::false_type{}, at, key0, tile * (KT / kGroup));
+        else tile_of(std::true_type{}, at, key0, tile * (KT / kGroup));
+    }
+    float l = fold_32_apart(l_run, AddOf());
+
+    if constexpr (KS > 1) {                      // the groups' results, joined in their order
+        float* const space = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        if (ksi > 0) {
+            float* mine = space + static_cast<size_t>((ksi - 1) * RB + rb) * 64 * (HD / 2 + 2) + lane;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mine[(d * 16 + e) * 64] = acc[d][e];
+            mine[HD / 2 * 64] = m_run;
+            mine[(HD / 2 + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (ksi > 0) return;
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+            const float* from_k = space + static_cast<size_t>((k - 1) * RB + rb) * 64 * (HD / 2 + 2) + lane;
+            const float m_k = from_k[HD / 2 * 64], l_k = from_k[(HD / 2 + 1) * 64];
+            const float m_new = fmaxf(m_run, m_k);
+            const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale2);
+            const float c = m_k == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_k - m_new) * scale2);
+            l = l * a + l_k * c;
+            m_run = m_new;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * a + from_k[(d * 16 + e) * 64] * c;
+        }
+    }
+    if (!valid) return;
+    const size_t row = static_cast<size_t>(token) * z.nq + head;
+    if (n_parts == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        T* const o = out + row * z.hd;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = d * 32 + e * 2 + lh * 4;
+                const float v[4] = {acc[d][e] * inv, acc[d][e + 1] * inv, acc[d][e + 2] * inv, acc[d][e + 3] * inv};
+                if (at < z.hd) write_quad(o + at, v);
+            }
+    } else {
+        const size_t mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
+        float* const o = part_o + mine * z.hd;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = d * 32 + e * 2 + lh * 4;
+                const float v[4] = {acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+                if (at < z.hd) write_quad(o + at, v);
+            }
+        if (lh == 0) {
+            part_ml[mine * 2] = m_run * scale2;
+            part_ml[mine * 2 + 1] = l;
+        }
+    }
+}
+
+// The parts of a request's keys joined, a wavefront per row: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A part that saw nothing weighs nothing, whatever it holds.
+template <typename T>
+__global__ __launch_bounds__(256) void tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                           const int32_t* __restrict__ q_start, const int32_t* __restrict__ q_len,
+                                                           const int32_t* __restrict__ kv_len, int nodes, int most_parts, int n_tokens, int nq, int hd, int chunk,
+                                                           unsigned magic_chunk, unsigned magic_heads, T* __restrict__ out) {
+    const int lane = threadIdx.x % kWave, w = blockIdx.x * 4 + threadIdx.x / kWave, b = blockIdx.y;
+    const int node = divided(w, nq, magic_heads), head = w - node * nq;
+    const int n = q_len[b], kv = kv_len[b];
+    const int parts = min(divided(max(kv, 1) - 1, chunk, magic_chunk) + 1, most_parts), token = q_start[b] + node;
+    if (node >= n || node >= nodes || parts < 2 || token < 0 || token >= n_tokens) return;
+    const size_t row = static_cast<size_t>(token) * nq + head, step = static_cast<size_t>(n_tokens) * nq;
+    float m_most = -INFINITY;
+    for (int p = lane; p < parts; p += kWave)
+        if (part_ml[(p * step + row) * 2 + 1] != 0.f) m_most = fmaxf(m_most, part_ml[(p * step + row) * 2]);
+    m_most = wave_max(m_most);
+    float total = 0.f, v[4] = {};
+    for (int p = 0; p < parts; ++p) {
+        const float m = part_ml[(p * step + row) * 2], l = part_ml[(p * step + row) * 2 + 1];
+        if (l == 0.f) continue;
+        const float share = __builtin_amdgcn_exp2f(m - m_most);
+        total = fmaf(l, share, total);
+        const float* o = part_o + (p * step + row) * hd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + i * kWave < hd) v[i] = fmaf(o[lane + i * kWave], share, v[i]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane + i * kWave < hd) out[row * hd + lane + i * kWave] = from_float<T>(v[i] * inv);
+}
+
+template <typename T, int HD, int RB, int KS, int KT, int NS>
+static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                       const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible, const int32_t* positions, TreeSizes z,
+                       int max_rows, hipStream_t s) {
+    constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS>();
+    static_assert(lds <= 160 * 1024, "a CU's LDS");
+    if (z.chunk % (KT * KS) != 0 || z.chunk > kMostGroups * kGroup) return EGPT_BAD_ARGUMENT;
+    z.blocks = (max_rows + 32 * RB - 1) / (32 * RB);
+    z.magic_blocks = magic_of(z.blocks);
+    const long long units = static_cast<long long>(z.n_seqs) * z.nkv * z.parts, grid = (units + 7) / 8 * 8 * z.blocks;
+    if (grid >= 1 << 27) return EGPT_UNSUPPORTED_SIZE;
+    auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
+    if (lds > 64 * 1024) {
+        static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+        if (!raised) return EGPT_UNSUPPORTED_SIZE;
+    }
+    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, q_start, block_table, static_cast<const T*>(qkv), visible, positions,
+                                                                   static_cast<const T*>(k_cache), static_cast<const T*>(v_cache), static_cast<T*>(out),
+                                                                   part_o, part_ml, z);
+    EGPT_CHECK_LAUNCH();
+    if (z.parts > 1) {
+        const int nodes = max_rows / z.group;
+        tree_combine_kernel<T><<<dim3((nodes * z.nq + 3) / 4, z.n_seqs), 256, 0, s>>>(part_o, part_ml, q_start, q_len, kv_len, nodes, z.parts, z.n_tokens, z.nq, z.hd,
+                                                                                 z.chunk, magic_of(z.chunk), magic_of(z.nq), static_cast<T*>(out));
+        EGPT_CHECK_LAUNCH();
+    }
+    return EGPT_OK;
+}
+
 }  // namespace egpt
 
 using namespace egpt;
@@ -148,4 +635,56 @@ extern "C" int egpt_tree_attention_generic(const void* qkv, void* out, const voi
     else launch(bf16_t{});
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
+}
+
+// shape: blocks of 32 rows that a workgroup takes, 1, 2, 4 or 8.
+extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache,
+                                   const int32_t* block_table, int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len,
+                                   const int32_t* kv_len, const long long* visible, const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv,
+                                   int hd, int page_size, float scale, int window, int max_q_len, int shape, int parts, int chunk, int dtype, void* stream) {
+    if (!qkv || !out || !k_cache || !v_cache || !block_table || !q_start || !q_len || !kv_len || !visible || (window > 0 && !positions))
+        return EGPT_BAD_ARGUMENT;
+    if (n_seqs <= 0 || n_tokens < 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || hd <= 0 || page_size <= 0 || table_width <= 0 || window < 0 ||
+        n_pages < 0 || max_q_len < 0 || dtype < 0 || dtype > 1 || parts <= 0 || chunk <= 0 || (parts > 1 && (!part_o || !part_ml)))
+        return EGPT_BAD_ARGUMENT;
+    const int size = dtype == 0 ? 4 : 2;
+    if (hd > kMaxTreeHead || hd * size % 16 != 0 || page_size % kGroup != 0 || max_q_len > 64 || nq > 65535 || n_seqs > 65535 ||
+        static_cast<long long>(hd) * page_size * size > 0x7fffffffLL || static_cast<long long>(table_width) * page_size > 0x7fffffLL * kGroup)
+        return EGPT_UNSUPPORTED_SIZE;
+    if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
+        return EGPT_UNSUPPORTED_SIZE;
+    if (n_tokens == 0 || max_q_len == 0) return EGPT_OK;
+    const int group = nq / nkv;
+    const TreeSizes z{table_width, n_pages, page_size, nq, nkv, hd, group, n_seqs, parts, chunk, 1, window, n_tokens,
+                      magic_of(parts), magic_of(nkv), 0u, magic_of(group), magic_of(page_size), magic_of(chunk), scale};
+    const int max_rows = max_q_len * group;
+#define EGPT_TREE(...) \
+    return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, positions, z, max_rows, \
+                                    static_cast<hipStream_t>(stream))
+    // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS)
+    if (dtype == 1 && hd <= 64) {
+        if (shape == 1) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);
+        if (shape == 2) EGPT_TREE(bf16_t, 64, 2, 2, 64, 2);
+        if (shape == 4) EGPT_TREE(bf16_t, 64, 4, 1, 64, 3);
+        if (shape == 8) EGPT_TREE(bf16_t, 64, 8, 1, 64, 3);
+    } else if (dtype == 1 && hd <= 128) {
+        if (shape == 1) EGPT_TREE(bf16_t, 128, 1, 4, 32, 2);
+        if (shape == 2) EGPT_TREE(bf16_t, 128, 2, 2, 64, 2);
+        if (shape == 4) EGPT_TREE(bf16_t, 128, 4, 1, 64, 2);
+        if (shape == 8) EGPT_TREE(bf16_t, 128, 8, 1, 64, 3);
+    } else if (dtype == 1) {
+        if (shape == 1) EGPT_TREE(bf16_t, 256, 1, 2, 32, 2);
+        if (shape == 4) EGPT_TREE(bf16_t, 256, 4, 1, 32, 3);
+    } else if (hd <= 64) {
+        if (shape == 1) EGPT_TREE(float, 64, 1, 4, 32, 2);
+        if (shape == 2) EGPT_TREE(float, 64, 2, 2, 32, 2);
+        if (shape == 4) EGPT_TREE(float, 64, 4, 1, 32, 3);
+    } else if (hd <= 128) {
+        if (shape == 1) EGPT_TREE(float, 128, 1, 2, 32, 2);
+        if (shape == 4) EGPT_TREE(float, 128, 4, 1, 32, 3);
+    } else {
+        if (shape == 4) EGPT_TREE(float, 256, 4, 1, 32, 2);
+    }
+#undef EGPT_TREE
+    return EGPT_BAD_ARGUMENT;
 }

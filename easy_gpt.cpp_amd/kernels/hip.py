@@ -112,6 +112,7 @@ class HipKernels(KernelBackend):
             "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
             "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
             "egpt_tree_attention_generic": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
+            "egpt_tree_attention": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, i, i, i, i, vp],
             "egpt_accept_drafts": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp],
             "egpt_keep_drafts": [vp, vp, vp, i, vp, vp, i, vp, i, i, i, i, i, i, i, i, vp],
             "egpt_gemm_gate_up_swiglu": [vp, vp, vp, i, i, i, i, i, vp],
@@ -2237,9 +2238,38 @@ class HipKernels(KernelBackend):
         self._here(qkv, out, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, positions if window else None)
         if t == 0 or b == 0:
             return
+        if hd * qkv.element_size() % 16 == 0 and page_size % 16 == 0 and not (qkv.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+            shape, parts, chunk = self._tree_shape(b, nkv, nq // nkv, hd, dt, max_q_len, max_kv_len)
+            part_o = part_ml = None
+            if parts > 1:
+                part_o = torch.empty((parts, t, nq, hd), dtype=_F32, device=qkv.device)
+                part_ml = torch.empty((parts, t, nq, 2), dtype=_F32, device=qkv.device)
+            self._run("egpt_tree_attention", qkv.data_ptr(), out.data_ptr(), self._ptr(part_o), self._ptr(part_ml), k_cache.data_ptr(), v_cache.data_ptr(),
+                      block_table.data_ptr(), width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
+                      positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), int(max_q_len), shape, parts,
+                      chunk, dt, self._stream())
+            return
         self._run("egpt_tree_attention_generic", qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
                   width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
                   positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), dt, self._stream())
+
+    @staticmethod
+    @functools.lru_cache(maxsize=4096)
+    def _tree_shape(b, nkv, group, hd, dt, max_q_len, max_kv_len) -> tuple[int, int, int]:
+        """(blocks of 32 rows to a workgroup, parts of the keys at most, keys of a part) of the matrix-core kernel."""
+        rows = max_q_len * group
+        shape = 1 if rows <= 32 else 2 if rows <= 64 else 4 if rows <= 128 else 8
+        if dt == 0 or hd > 128:
+            shape = min(shape, 4)
+            if shape == 2 and hd > (64 if dt == 0 else 128):
+                shape = 4
+            if shape < 4 and dt == 0 and hd > 128:
+                shape = 4
+        units = b * nkv * -(-rows // (32 * shape))
+        most = -(-max_kv_len // 128)
+        parts = max(1, min(512 // units, most, 64), -(-max_kv_len // 8192))
+        chunk = max(1, -(-most // parts)) * 128
+        return shape, max(1, -(-max_kv_len // chunk)), chunk
 
     def accept_drafts(self, tokens, parents, sampled, q_start, q_len):
         t, b = tokens.shape[0], q_len.shape[0]
