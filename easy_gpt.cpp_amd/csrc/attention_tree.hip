@@ -15,6 +15,8 @@
 namespace egpt {
 
 constexpr int kMaxTreeHead = 256;
+constexpr float kSlack = 8.0f;                   // how far, in powers of two, a row's maximum may run ahead of the one in use
+constexpr int kMostParts = 64;                   // of a request's keys: a lane each where they are joined
 
 // One row's view of the keys: the tokens before the tree from `lo` on, and the nodes of its bits.
 struct TreeRow {
@@ -158,56 +160,37 @@ __device__ __forceinline__ f32x16 product_of(u32x4 a, u32x4 b, f32x16 c) {
     }
 }
 
-// Two bfloat16 numbers or a float32 as bits, by integer arithmetic (comparisons of every element leave the scalar registers no room): at the top bit of
-// each number whether it is an infinity or a NaN, and whether it is a NaN.
-template <typename T>
-__device__ __forceinline__ unsigned not_finite(unsigned x) {
-    if constexpr (sizeof(T) == 2) return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-    else return ((x & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-}
-template <typename T>
-__device__ __forceinline__ unsigned fraction_of(unsigned x) {
-    if constexpr (sizeof(T) == 2) return (((x & 0x007f007fu) + 0x007f007fu) & 0x00800080u) << 8;
-    else return ((x & 0x007fffffu) + 0x007fffffu) << 8 & 0x80000000u;
-}
-// All ones in the numbers whose top bit is set, and the number 1 there.
-template <typename T>
-__device__ __forceinline__ unsigned filled(unsigned top) {
-    if constexpr (sizeof(T) == 2) return (top >> 15) * 0xffffu;
-    else return static_cast<unsigned>(static_cast<int>(top) >> 31);
-}
-template <typename T>
-__device__ __forceinline__ unsigned one_where(unsigned top) { return filled<T>(top) & (sizeof(T) == 2 ? 0x3f803f80u : 0x3f800000u); }
 // All ones if bit `at` of x is set.
 __device__ __forceinline__ unsigned bit_filled(unsigned x, int at) { return static_cast<unsigned>(static_cast<int>(x << (31 - at)) >> 31); }
 
 constexpr int kGroup = 16;                       // keys that a load's base is found for: never more than a page's
-constexpr int kMostGroups = 512;                 // of a workgroup's part
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"        // (m0 is a reserved register; nothing else here uses it)
-// 16 bytes a lane from byte `offset` of a resource to LDS, at address `to` (the same for the whole wavefront) + 16 x lane; zeros past its end.
-__device__ __forceinline__ void load_1k(r_i32x4 resource, int offset, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(resource)
+// 16 bytes a lane from byte `offset` + `more` of a resource to LDS, at address `to` (the same for the whole wavefront) + 16 x lane; zeros past its end.
+__device__ __forceinline__ void load_1k(r_i32x4 resource, int offset, int more, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(resource),
+                 "s"(more)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
-
 struct TreeSizes {
-    int table_width, n_pages, page_size, nq, nkv, hd, group, n_seqs, parts, chunk, blocks, window, n_tokens;
-    unsigned magic_parts, magic_nkv, magic_blocks, magic_group, magic_page, magic_chunk;
+    int n_pages, page_size, nq, hd, group, n_seqs, window, n_tokens;
+    unsigned magic_group, magic_page, magic_chunk;
     float scale;
 };
 
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 constexpr int tree_lds() {
     constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = (KS - 1) * RB * 64 * (HD / 2 + 2) * 4;
-    return (stages > join ? stages : join) + kMostGroups * 8 + 16;
+    return stages > join ? stages : join;
 }
 
+// (the first 14 words of the arguments arrive with the wavefronts: all that the first trip to memory needs)
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1) void tree_attention_kernel(
-    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start, const int32_t* __restrict__ block_table,
+    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int blocks, unsigned magic_blocks,
+    int parts, unsigned magic_parts, int nkv, unsigned magic_nkv, int table_width, int chunk, const int32_t* __restrict__ q_start,
     const T* __restrict__ qkv, const long long* __restrict__ visible, const int32_t* __restrict__ positions, const T* __restrict__ k_cache,
     const T* __restrict__ v_cache, T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml, TreeSizes z) {
     constexpr int SZ = sizeof(T);
@@ -218,41 +201,115 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     constexpr int OWN = LOADS > PER_GROUP ? LOADS / PER_GROUP : 1, EACH = LOADS > PER_GROUP ? PER_GROUP : LOADS;
     constexpr int STEPS = SZ == 2 ? 2 : 4;                       // second products of a block of 32 keys: 32 bytes of a feature each
     static_assert(LOADS >= 1 && HALF % (1024 * RB) == 0 && OWN * EACH == LOADS, "every wavefront loads as much");
+    static_assert(kWave * kGroup % (KT * KS) == 0, "the 64 groups that a wavefront has the pages of are whole rounds");
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr int SPACE = tree_lds<T, HD, RB, KS, KT, NS>() - kMostGroups * 8 - 16;
-    int2* const s_place = reinterpret_cast<int2*>(smem + SPACE);          // page and offset of every group of the part
-    int* const s_missing = reinterpret_cast<int*>(smem + SPACE + kMostGroups * 8);
     const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 32, lh = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), rb = wave % RB, ksi = wave / RB;
 
     // Which part of which request and kv head, and which block of its rows.  Workgroups go to the eight dies in turn: the blocks of rows that read the same
     // keys follow each other on one of them.
     const int slot = blockIdx.x / 8;
-    const int unit0 = divided(slot, z.blocks, z.magic_blocks);
-    const int block = slot - unit0 * z.blocks, unit = unit0 * 8 + blockIdx.x % 8;
-    const int pair = divided(unit, z.parts, z.magic_parts), part = unit - pair * z.parts;
-    const int b = divided(pair, z.nkv, z.magic_nkv), kvh = pair - b * z.nkv;
+    const int unit0 = divided(slot, blocks, magic_blocks);
+    const int block = slot - unit0 * blocks, unit = unit0 * 8 + blockIdx.x % 8;
+    const int pair = divided(unit, parts, magic_parts), part = unit - pair * parts;
+    const int b = divided(pair, nkv, magic_nkv), kvh = pair - b * nkv;
     if (b >= z.n_seqs) return;
-    const int n = q_len[b], rows = n * z.group, row0 = block * 32 * RB;
+    const int n = q_len[b], kv_all = kv_len[b], qs = q_start[b];
+    const int from = part * chunk;
+    // The pages of 64 groups of keys, a lane each, asked for before it is known how many keys there are; the next 64 while these are walked.
+    const int32_t* const table = block_table + static_cast<size_t>(b) * table_width;
+    struct Places {
+        int page, off;                                           // (page -1: none)
+    };
+    auto places_from = [&](int first_key) {
+        const int key = min(first_key + lane * kGroup, table_width * z.page_size - 1), at = divided(key, z.page_size, z.magic_page);
+        const int page = table[at];
+        return Places{page >= z.n_pages ? -1 : page, key - at * z.page_size};
+    };
+    Places here = places_from(from);
+    const int rows = n * z.group, row0 = block * 32 * RB;
     if (row0 >= rows) return;
-    const int kv_all = kv_len[b], before = kv_all - n, kv = min(kv_all, z.table_width * z.page_size);
-    const int qs = q_start[b];
-    const int n_parts = min(divided(max(kv_all, 1) - 1, z.chunk, z.magic_chunk) + 1, z.parts);
+    const int before = kv_all - n, kv = min(kv_all, table_width * z.page_size);
+    const int n_parts = min(divided(max(kv_all, 1) - 1, chunk, z.magic_chunk) + 1, parts);
     if (part >= n_parts) return;
+    const int to = min(kv, from + chunk);
+    const int groups = to > from ? (to - from + kGroup - 1) / kGroup : 0;
+
+    const int key_bytes = z.hd * SZ;
+    const size_t head_bytes = static_cast<size_t>(z.page_size) * key_bytes, page_bytes = head_bytes * nkv;
+    const char* const k_head = reinterpret_cast<const char*>(k_cache) + kvh * head_bytes;
+    const char* const v_head = reinterpret_cast<const char*>(v_cache) + kvh * head_bytes;
+    // A wavefront's loads of a tile: EACH of a group's PER_GROUP, of OWN groups.  Load u has the group's keys from u * (1024 / ROWB) on, and the values' features from
+    // u * (64 / SZ) on; what differs between a wavefront's loads is a scalar offset and, in the exchange of a key's pieces, bits of its number above the lane's.
+    constexpr int row_swap = PIECES >= 16 ? 15 : 7, KEYS = 1024 / ROWB;
+    const int first_load = rb * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
+    auto swap_of = [](int key) { return (SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key) & row_swap; };      // bfloat16: bits 2 and 3 exchanged
+    const int k_at = lane / PIECES * key_bytes, k_place = lane % PIECES ^ swap_of(lane / PIECES);
+    const int v_at = lane / SZ * z.page_size * SZ + (SZ == 2 ? lane % 2 : (lane % 4) ^ (lane / SZ >> 2 & 3)) * 16;       // (features past the head's lie past the resource's end)
+    const int n_tiles = (groups * kGroup + KT - 1) / KT, rounds = (n_tiles + KS - 1) / KS;
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)smem));
+    // (`places`: those of the 64 groups that the round's keys are among)
+    auto load_tile = [&](int round, const Places& places) {
+        const unsigned base = lds0 + (round % NS * KS + ksi) * TILE + first_load * 1024;
+        const int g0 = (round * KS + ksi) * (KT / kGroup) + group_first;
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int page = g0 + o < groups ? __builtin_amdgcn_readlane(places.page, (g0 + o) % kWave) : -1;
+            const int off = __builtin_amdgcn_readlane(places.off, (g0 + o) % kWave);
+            const size_t at = static_cast<size_t>(max(page, 0)) * page_bytes;
+            const r_i32x4 keys = buffer_of(k_head + at + static_cast<size_t>(off) * key_bytes, page < 0 ? 0 : kGroup * key_bytes);
+            const r_i32x4 values = buffer_of(v_head + at + static_cast<size_t>(off) * SZ, page < 0 ? 0 : head_bytes - static_cast<size_t>(off) * SZ);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                const int piece = (k_place ^ swap_of((load_first + j) * KEYS)) * 16;
+                load_1k(keys, piece < key_bytes ? k_at + piece : kNowhere, (load_first + j) * KEYS * key_bytes, base + (o * PER_GROUP + j) * 1024);
+            }
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) load_1k(values, v_at, (load_first + j) * 64 * z.page_size, base + HALF + (o * PER_GROUP + j) * 1024);
+        }
+    };
+    constexpr int AHEAD = kWave * kGroup / (KT * KS);            // rounds that the places of 64 groups serve
+    static_assert(AHEAD >= NS, "the tiles ahead lie within the next places");
 
     // this lane's row
     const int r = row0 + rb * 32 + lr;
-    const bool valid = r < rows && qs >= 0 && qs + divided(r, z.group, z.magic_group) < z.n_tokens;
-    const int node = valid ? divided(r, z.group, z.magic_group) : 0;
-    const int head = kvh * z.group + (valid ? r - node * z.group : 0);
+    const int node_at = divided(r, z.group, z.magic_group);
+    const bool valid = r < rows && qs >= 0 && qs + node_at < z.n_tokens;
+    const int node = valid ? node_at : 0, head = kvh * z.group + (valid ? r - node * z.group : 0);
     const int token = qs + node;
-    unsigned long long bits = valid ? static_cast<unsigned long long>(visible[token]) : 0ull;
-    int lo = valid && z.window > 0 ? min(max(0, positions[token] - z.window + 1), max(before, 0)) : 0;
-    if (!valid) lo = 0x7fffffff;
-    const int key_bytes = z.hd * SZ;
+    // the first round: with a window the one that has the first key that any row of the workgroup sees
+    int lo = valid ? 0 : 0x7fffffff, first_round = 0, all_see = 0;       // all_see: from which key on all rows see everything before the tree
+    if (z.window > 0) {
+        __shared__ int s_least, s_most;
+        if (tid == 0) {
+            s_least = 0x7fffffff;
+            s_most = 0;
+        }
+        __syncthreads();
+        if (valid) {
+            lo = min(max(0, positions[token] - z.window + 1), max(before, 0));
+            atomicMin(&s_least, lo);
+            atomicMax(&s_most, lo);
+        }
+        __syncthreads();
+        first_round = __builtin_amdgcn_readfirstlane(max(0, min(s_least, max(before, 0)) - from) / (KT * KS));
+        all_see = __builtin_amdgcn_readfirstlane(s_most);
+    }
+    int window_of = 0;                                           // `here` has the places of groups [64 window_of, 64 window_of + 64)
+    if (first_round >= AHEAD) {
+        window_of = first_round / AHEAD;
+        here = places_from(from + window_of * kWave * kGroup);
+    }
+    Places next = places_from(from + (window_of + 1) * kWave * kGroup);
+    auto load_round = [&](int round) { load_tile(round, round / AHEAD == window_of ? here : next); };
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+        if (first_round + i < rounds) load_round(first_round + i);
+
+    const unsigned long long bits = valid ? static_cast<unsigned long long>(visible[token]) : 0ull;
     u32x4 q[KC];
     {
-        const char* qp = reinterpret_cast<const char*>(qkv + static_cast<size_t>(token) * (z.nq + 2 * z.nkv) * z.hd + head * z.hd);
+        const char* qp = reinterpret_cast<const char*>(qkv + static_cast<size_t>(token) * (z.nq + 2 * nkv) * z.hd + head * z.hd);
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
             const int at = i * 32 + lh * 16;
@@ -260,69 +317,6 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             if (z.scale < 0.f) q[i] ^= SZ == 2 ? 0x80008000u : 0x80000000u;        // (the greatest score is the greatest product then as well)
         }
     }
-    // the keys of this part that the workgroup's rows see: from the lowest window's first on
-    int lo_wave_least = 0, lo_wave_most = 0;
-    if (z.window > 0) {
-        float least = valid ? static_cast<float>(lo) : 3.0e38f, most = valid ? static_cast<float>(lo) : 0.f;      // (places are below 2^24, or the bounds a little wider)
-        least = -wave_max(-least);
-        most = wave_max(most);
-        lo_wave_least = least > 2.0e9f ? 0 : max(0, static_cast<int>(least) - (least > 16777216.f ? 256 : 0));
-        lo_wave_most = static_cast<int>(fminf(most, 2.0e9f)) + (most > 16777216.f ? 256 : 0);
-    }
-    const int from = part * z.chunk, to = min(kv, from + z.chunk);
-    const int groups = to > from ? (to - from + kGroup - 1) / kGroup : 0;
-    {
-        if (tid == 0) *s_missing = 0;
-        __syncthreads();
-        const int32_t* table = block_table + static_cast<size_t>(b) * z.table_width;
-        for (int i = tid; i < groups; i += 64 * RB * KS) {
-            const int key = from + i * kGroup, at = divided(key, z.page_size, z.magic_page);
-            int page = table[at];
-            if (page < 0 || page >= z.n_pages) {
-                page = -1;
-                *s_missing = 1;                                  // (some rows' tiles may lie before their window, where pages have been given back)
-            }
-            s_place[i] = int2{page, key - at * z.page_size};
-        }
-        __syncthreads();
-    }
-    const bool missing = *s_missing != 0;
-
-    const size_t head_bytes = static_cast<size_t>(z.page_size) * key_bytes, page_bytes = head_bytes * z.nkv;
-    const char* const k_head = reinterpret_cast<const char*>(k_cache) + kvh * head_bytes;
-    const char* const v_head = reinterpret_cast<const char*>(v_cache) + kvh * head_bytes;
-    const int row_swap = PIECES >= 16 ? 15 : 7;
-    const int first_load = rb * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
-    int k_at[EACH], v_at[EACH];
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const int u = load_first + j;
-        const int key = u * (1024 / ROWB) + lane / PIECES;                   // of the group's 16
-        const int order = SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key;       // bits 2 and 3 exchanged
-        const int piece = (lane % PIECES) ^ (order & row_swap);
-        k_at[j] = piece * 16 < key_bytes ? key * key_bytes + piece * 16 : kNowhere;
-        const int d = u * (64 / SZ) + lane / SZ;
-        const int v_piece = SZ == 2 ? lane % 2 : (lane % 4) ^ (d >> 2 & 3);
-        v_at[j] = d < z.hd ? d * z.page_size * SZ + v_piece * 16 : kNowhere;
-    }
-    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)smem));
-    const int n_tiles = (groups * kGroup + KT - 1) / KT, rounds = (n_tiles + KS - 1) / KS;
-    auto load_tile = [&](int round) {
-        const unsigned base = lds0 + (round % NS * KS + ksi) * TILE + first_load * 1024;
-        const int g0 = (round * KS + ksi) * (KT / kGroup) + group_first;
-#pragma unroll
-        for (int o = 0; o < OWN; ++o) {
-            const int2 place = g0 + o < groups ? s_place[g0 + o] : int2{-1, 0};
-            const int page = __builtin_amdgcn_readfirstlane(place.x), off = __builtin_amdgcn_readfirstlane(place.y);
-            const size_t at = static_cast<size_t>(max(page, 0)) * page_bytes;
-            const r_i32x4 keys = buffer_of(k_head + at + static_cast<size_t>(off) * key_bytes, page < 0 ? 0 : kGroup * key_bytes);
-            const r_i32x4 values = buffer_of(v_head + at + static_cast<size_t>(off) * SZ, page < 0 ? 0 : head_bytes - static_cast<size_t>(off) * SZ);
-#pragma unroll
-            for (int j = 0; j < EACH; ++j) load_1k(keys, k_at[j], base + (o * PER_GROUP + j) * 1024);
-#pragma unroll
-            for (int j = 0; j < EACH; ++j) load_1k(values, v_at[j], base + HALF + (o * PER_GROUP + j) * 1024);
-        }
-    };
 
     f32x16 acc[DB];
 #pragma unroll
@@ -330,7 +324,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
-    const float scale2 = fabsf(z.scale) * 1.4426950408889634f;          // exponentials are taken to the base 2
+    const float scale2 = fabsf(z.scale) * 1.4426950408889634f;   // exponentials are taken to the base 2
     const int my_key = SZ == 2 ? (lr & 3) | (lr >> 1 & 4) | (lr << 1 & 8) | (lr & 16) : lr;
     const int k_row = my_key * ROWB, k_piece = (lh ^ (lr & row_swap)) * 16;
     const int v_row = lr * kGroup * SZ + (SZ == 2 ? lh * 16 : ((lh ^ (lr >> 2 & 3)) * 16));
@@ -341,10 +335,69 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
         const int row = SZ == 2 ? v_row : v_row ^ ((step % 2) * 32);
         return piece_at(tile + HALF + (g * HD + d * 32) * kGroup * SZ + row);
     };
-    // A tile.  MASKED: its scores are compared with what the row sees, and its values may hold numbers that are none, which rows that do not see them are kept from.
-    auto tile_of = [&](auto masked, const char* tile, int key0, int group0) {
+    // A tile with values that are no finite numbers, some of them of nodes that not every row sees: a row's weight for such a key is zero, and zero times
+    // an infinity is none.  So one key after the other, on the vector pipe, left out where it is not seen.  (Rare, and slow: registers that it held would be the other tiles'.)
+    auto strange_tile = [&](const char* tile, int key0, const Places& places) {
+#pragma unroll 1
+        for (int key = 0; key < KT; ++key) {
+            const int j = key0 + key;
+            if (j >= to) break;
+            if (__builtin_amdgcn_readlane(places.page, (j - from) / kGroup % kWave) < 0) continue;
+            const bool sees = valid && (j < before ? j >= lo : j - before < 64 && (bits >> (j - before) & 1ull) != 0);
+            if (!__any(sees)) continue;
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < KC; ++i) {
+                const u32x4 k = *reinterpret_cast<const u32x4*>(tile + key * ROWB + (((2 * i + lh) ^ swap_of(key)) * 16));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (SZ == 2) {
+                        dot = fmaf(__uint_as_float(k[e] << 16), __uint_as_float(q[i][e] << 16), dot);
+                        dot = fmaf(__uint_as_float(k[e] & 0xffff0000u), __uint_as_float(q[i][e] & 0xffff0000u), dot);
+                    } else {
+                        dot = fmaf(__uint_as_float(k[e]), __uint_as_float(q[i][e]), dot);
+                    }
+                }
+            }
+            dot = fold_32_apart(dot, AddOf());
+            const float m_new = sees ? fmaxf(m_run, dot) : m_run, m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_use) * scale2), w = __builtin_amdgcn_exp2f((dot - m_use) * scale2);
+            m_run = m_new;
+            l_run = l_run * alpha + (sees && lh == 0 ? w : 0.f);             // (the halves' sums are added up in the end)
+            const char* const values = tile + HALF + key / kGroup * HD * kGroup * SZ;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int feature = d * 32 + e / 4 * 8 + lh * 4 + e % 4, in = key % kGroup;
+                    float v;
+                    if constexpr (SZ == 2) v = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(values + feature * 32 + in * 2)) << 16);
+                    else v = *reinterpret_cast<const float*>(values + feature * 64 + ((in / 4) ^ (feature >> 2 & 3)) * 16 + in % 4 * 4);
+                    const float scaled = acc[d][e] * alpha;
+                    acc[d][e] = sees ? fmaf(w, v, scaled) : scaled;
+                }
+        }
+    };
+    // A tile.  MASKED: its scores are compared with what the row sees.
+    auto tile_of = [&](auto masked, const char* tile, int key0, const Places& places) {
         constexpr bool MASKED = decltype(masked)::value;
         constexpr int R = SZ == 2 ? 8 : 4;                                      // neighbouring keys of a lane
+        if constexpr (MASKED) {
+            // whether any value is no finite number: their products with zeros are zeros unless it is
+            f32x16 probe;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) probe[e] = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) probe = product_of<T>(values_at(tile, kb, step, d), u32x4{0u, 0u, 0u, 0u}, probe);
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum += probe[e];
+            if (__builtin_expect(__any(sum != 0.f), 0)) return strange_tile(tile, key0, places);
+        }
         f32x16 s[KB];
         unsigned sees[KB];
 #pragma unroll
@@ -360,11 +413,11 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
                 const int skip = lo - k0;
                 if (skip > 0) early = skip >= 32 ? 0u : early & (0xffffffffu << skip);
                 unsigned all = static_cast<unsigned>(w) | early;
-                const int end = kv - k0;
+                const int end = to - k0;
                 if (end < 32) all = end > 0 ? all & ((1u << end) - 1u) : 0u;
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
-                    if (group0 + kb * 2 + g >= groups || s_place[group0 + kb * 2 + g].x < 0) all &= g == 0 ? 0xffff0000u : 0x0000ffffu;
+                    if (__builtin_amdgcn_readlane(places.page, ((k0 - from) / kGroup + g) % kWave) < 0) all &= g == 0 ? 0xffff0000u : 0x0000ffffu;
                 if (!valid) all = 0u;
                 sees[kb] = all >> (lh * R);
 #pragma unroll
@@ -374,13 +427,15 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
                 }
             }
         }
-        float mx = s[0][0];
+        float mx = s[0][0];          // (two at a time are one instruction)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+            for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, s[kb][e]), s[kb][e + 1]);
         mx = fold_32_apart(mx, MaxOf());
-        if (__any(mx > m_run)) {
+        // The maximum that exponentials are taken against follows a row's once that has grown by more than 2^kSlack: they may reach 2^kSlack meanwhile, which
+        // float32 sums do not mind, nor bfloat16, as near at any magnitude; and the sums are rescaled a few times a context and not every few tiles.
+        if (__any((mx - m_run) * scale2 > kSlack || (m_run == -INFINITY && mx > m_run))) {
             const float m_new = fmaxf(m_run, mx);
             const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale2);
             l_run *= alpha;
@@ -404,87 +459,65 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
                 sum += p;
             }
             l_run += sum;
-            [[maybe_unused]] unsigned strange = 0u;
+        }
+        auto weights_of = [&](int kb, int step) {
+            u32x4 p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (SZ == 2) p[e] = bf16_pair(s[kb][step * 8 + 2 * e], s[kb][step * 8 + 2 * e + 1]);
+                else p[e] = __float_as_uint(s[kb][step * 4 + e]);
+            }
+            return p;
+        };
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int step = 0; step < STEPS; ++step) {
-                u32x4 p;
+                const u32x4 p = weights_of(kb, step);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (SZ == 2) p[e] = bf16_pair(s[kb][step * 8 + 2 * e], s[kb][step * 8 + 2 * e + 1]);
-                    else p[e] = __float_as_uint(s[kb][step * 4 + e]);
-                }
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    u32x4 v = values_at(tile, kb, step, d);
-                    if constexpr (MASKED) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const unsigned it = not_finite<T>(v[e]);
-                            strange |= it;
-                            v[e] &= ~filled<T>(it);
-                        }
-                    }
-                    acc[d] = product_of<T>(v, p, acc[d]);
-                }
+                for (int d = 0; d < DB; ++d) acc[d] = product_of<T>(values_at(tile, kb, step, d), p, acc[d]);
             }
-            if constexpr (MASKED) {
-                // Values that are no finite numbers, left out above: how many infinities of either sign (a NaN is both) each row sees, by the same products of ones,
-                // and what they make of the sum.
-                if (__any(strange != 0u)) {
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        f32x16 up, down;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) up[e] = down[e] = 0.f;
-#pragma unroll
-                        for (int step = 0; step < STEPS; ++step) {
-                            const u32x4 v = values_at(tile, kb, step, d);
-                            u32x4 seen, above, below;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const unsigned it = not_finite<T>(v[e]), nan = fraction_of<T>(v[e]);
-                                above[e] = one_where<T>(it & (nan | ~v[e]));
-                                below[e] = one_where<T>(it & (nan | v[e]));
-                                if constexpr (SZ == 2)
-                                    seen[e] = (bit_filled(sees[kb], step * 16 + 2 * e) & 0x3f80u) | (bit_filled(sees[kb], step * 16 + 2 * e + 1) & 0x3f800000u);
-                                else seen[e] = bit_filled(sees[kb], step * 8 + e) & 0x3f800000u;
-                            }
-                            up = product_of<T>(above, seen, up);
-                            down = product_of<T>(below, seen, down);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[d][e] += up[e] * 3.0e38f * 3.0e38f - down[e] * 3.0e38f * 3.0e38f;      // (0 or an infinity each)
-                    }
-                }
-            }
-        }
     };
 
-    // (tiles before every row's window are not loaded)
-    const int lo_block = z.window > 0 ? max(0, lo_wave_least) : 0;
-    int first_round = 0;
-    if (z.window > 0) {
-        __shared__ int s_least[8];
-        if (lane == 0) s_least[wave] = row0 + rb * 32 < rows ? lo_block : 0x7fffffff;
-        __syncthreads();
-        int least = 0x7fffffff;
-        for (int w = 0; w < RB * KS; ++w) least = min(least, s_least[w]);
-        first_round = max(0, min(least, before) - from) / (KT * KS);
-    }
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i)
-        if (first_round + i < rounds) load_tile(first_round + i);
-    for (int round = first_round; round < rounds; ++round) {
+    // Rounds whose keys every row sees, all before the tree, behind all windows and in pages, go without masks; they lie together.  (One loop that asked every
+    // time would carry the accumulators from one kind's registers to the other's.)
+    auto begin_round = [&](int round) {
         // this wavefront's loads of the tile are there when no more than those of the later ones are on their way; then everybody's
         if (round + NS - 1 <= rounds) arrived<(NS - 2) * 2 * LOADS>();
         else arrived<0>();
         __syncthreads();
-        if (round + NS - 1 < rounds) load_tile(round + NS - 1);
-        const int tile = round * KS + ksi, key0 = from + tile * KT;
-        if (tile >= n_tiles) continue;
-        const char* const at = smem + (round % NS * KS + ksi) * TILE;
-        if (!missing && key0 + KT <= min(before, kv) && key0 >= lo_wave_most) tile_of(std::false_type{}, at, key0, tile * (KT / kGroup));
-        else tile_of(std::true_type{}, at, key0, tile * (KT / kGroup));
+        if (round + NS - 1 < rounds) load_round(round + NS - 1);
+    };
+    auto tile_at = [&](int round) { return smem + (round % NS * KS + ksi) * TILE; };
+    auto gone_here = [&]() {
+        const int key = from + (window_of * kWave + lane) * kGroup;
+        return __any(here.page < 0 && key < before && key + kGroup > all_see) != 0;
+    };
+    auto end_round = [&](int round) {
+        if ((round + 1) % AHEAD != 0) return false;
+        here = next;
+        ++window_of;
+        if ((window_of + 1) * AHEAD < rounds) next = places_from(from + (window_of + 1) * kWave * kGroup);
+        return gone_here();
+    };
+    constexpr int ROUND = KT * KS;
+    const int open_end = (min(before, to) - from) / ROUND;
+    int round = first_round, stop = min(rounds, max(first_round, (all_see - from + ROUND - 1) / ROUND));
+    bool gone = gone_here();
+    for (;;) {
+        for (; round < stop; ++round) {
+            begin_round(round);
+            const int tile = round * KS + ksi;
+            if (tile < n_tiles) tile_of(std::true_type{}, tile_at(round), from + tile * KT, here);
+            end_round(round);
+        }
+        if (round >= rounds) break;
+        for (; round < open_end && !gone; ++round) {
+            begin_round(round);
+            tile_of(std::false_type{}, tile_at(round), from + (round * KS + ksi) * KT, here);
+            gone = end_round(round);
+        }
+        stop = rounds;
     }
     float l = fold_32_apart(l_run, AddOf());
 
@@ -519,92 +552,104 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     }
     if (!valid) return;
     const size_t row = static_cast<size_t>(token) * z.nq + head;
-    if (n_parts == 1) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        T* const o = out + row * z.hd;
+    const bool whole = n_parts == 1;
+    const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+    const size_t mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int at = d * 32 + e * 2 + lh * 4;
-                const float v[4] = {acc[d][e] * inv, acc[d][e + 1] * inv, acc[d][e + 2] * inv, acc[d][e + 3] * inv};
-                if (at < z.hd) write_quad(o + at, v);
-            }
-    } else {
-        const size_t mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
-        float* const o = part_o + mine * z.hd;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int at = d * 32 + e * 2 + lh * 4;
-                const float v[4] = {acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
-                if (at < z.hd) write_quad(o + at, v);
-            }
-        if (lh == 0) {
-            part_ml[mine * 2] = m_run * scale2;
-            part_ml[mine * 2 + 1] = l;
+        for (int e = 0; e < 16; e += 4) {
+            const int at = d * 32 + e * 2 + lh * 4;
+            const float v[4] = {acc[d][e] * inv, acc[d][e + 1] * inv, acc[d][e + 2] * inv, acc[d][e + 3] * inv};
+            if (at >= z.hd) continue;
+            if (whole) write_quad(out + row * z.hd + at, v);
+            else write_quad(part_o + mine * z.hd + at, v);
         }
+    if (!whole && lh == 0) {
+        part_ml[mine * 2] = m_run * scale2;
+        part_ml[mine * 2 + 1] = l;
     }
 }
 
-// The parts of a request's keys joined, a wavefront per row: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A part that saw nothing weighs nothing, whatever it holds.
+// The parts of a request's keys joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A wavefront has as many rows as it has times hd / 4 lanes; lane p of each
+// (at most 64 parts) takes part p's maximum and sum, so that the weights of all are known after one trip, and the parts' sums come kAhead at a time.  A part
+// that saw nothing weighs nothing, whatever it holds.
 template <typename T>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                                                           const int32_t* __restrict__ q_start, const int32_t* __restrict__ q_len,
-                                                           const int32_t* __restrict__ kv_len, int nodes, int most_parts, int n_tokens, int nq, int hd, int chunk,
-                                                           unsigned magic_chunk, unsigned magic_heads, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start,
+                                                           const float* __restrict__ part_ml, const float* __restrict__ part_o, int chunk, unsigned magic_chunk,
+                                                           int nq, unsigned magic_heads, int nodes, int most_parts, int n_tokens, int hd, T* __restrict__ out) {
+    constexpr int kAhead = 8;
     const int lane = threadIdx.x % kWave, w = blockIdx.x * 4 + threadIdx.x / kWave, b = blockIdx.y;
     const int node = divided(w, nq, magic_heads), head = w - node * nq;
-    const int n = q_len[b], kv = kv_len[b];
-    const int parts = min(divided(max(kv, 1) - 1, chunk, magic_chunk) + 1, most_parts), token = q_start[b] + node;
+    const int n = q_len[b], kv = kv_len[b], token = q_start[b] + node;
+    const int parts = min(divided(max(kv, 1) - 1, chunk, magic_chunk) + 1, most_parts);
     if (node >= n || node >= nodes || parts < 2 || token < 0 || token >= n_tokens) return;
     const size_t row = static_cast<size_t>(token) * nq + head, step = static_cast<size_t>(n_tokens) * nq;
-    float m_most = -INFINITY;
-    for (int p = lane; p < parts; p += kWave)
-        if (part_ml[(p * step + row) * 2 + 1] != 0.f) m_most = fmaxf(m_most, part_ml[(p * step + row) * 2]);
-    m_most = wave_max(m_most);
-    float total = 0.f, v[4] = {};
-    for (int p = 0; p < parts; ++p) {
-        const float m = part_ml[(p * step + row) * 2], l = part_ml[(p * step + row) * 2 + 1];
-        if (l == 0.f) continue;
-        const float share = __builtin_amdgcn_exp2f(m - m_most);
-        total = fmaf(l, share, total);
-        const float* o = part_o + (p * step + row) * hd;
+    const int quads = hd / 4, halves = quads <= 32 ? 2 : 1;      // (heads of up to 128: two parts at a time, 32 lanes each)
+    const int half = halves == 2 ? lane / 32 : 0, quad = halves == 2 ? lane % 32 : lane;
+    const int at = min(quad, quads - 1) * 4;
+    const float* const from = part_o + row * hd + at;
+    float v[kAhead][4];
+    auto ask = [&](int p0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + i * kWave < hd) v[i] = fmaf(o[lane + i * kWave], share, v[i]);
+        for (int i = 0; i < kAhead; ++i) read_quad(from + min(p0 + i * halves + half, parts - 1) * step * hd, v[i]);
+    };
+    ask(0);
+    const size_t mine = (min(lane, parts - 1) * step + row) * 2;
+    const float m = part_ml[mine], l = lane < parts ? part_ml[mine + 1] : 0.f;
+    const float m_most = wave_max(l != 0.f ? m : -INFINITY);
+    const float weight = l != 0.f ? __builtin_amdgcn_exp2f(m - m_most) : 0.f;
+    const float total = wave_sum(weight * l);
+    const unsigned long long some = __ballot(l != 0.f);
+    float sum[4] = {};
+    for (int p0 = 0;;) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int p = p0 + i * halves + half;
+            const float share = __shfl(weight, p % kWave, kWave);
+            if (p < parts && (some >> (p % kWave) & 1ull)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[i][e], share, sum[e]);
+            }
+        }
+        p0 += kAhead * halves;
+        if (p0 >= parts) break;
+        ask(p0);
     }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    if (halves == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + i * kWave < hd) out[row * hd + lane + i * kWave] = from_float<T>(v[i] * inv);
+        for (int e = 0; e < 4; ++e) sum[e] = fold_32_apart(sum[e], AddOf());
+    }
+    if (half != 0 || quad >= quads) return;
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    const float o[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+    write_quad(out + row * hd + at, o);
 }
 
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
-                       const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible, const int32_t* positions, TreeSizes z,
-                       int max_rows, hipStream_t s) {
+                       int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
+                       const int32_t* positions, const TreeSizes& z, int nkv, int parts, int chunk, int max_rows, hipStream_t s) {
     constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS>();
-    static_assert(lds <= 160 * 1024, "a CU's LDS");
-    if (z.chunk % (KT * KS) != 0 || z.chunk > kMostGroups * kGroup) return EGPT_BAD_ARGUMENT;
-    z.blocks = (max_rows + 32 * RB - 1) / (32 * RB);
-    z.magic_blocks = magic_of(z.blocks);
-    const long long units = static_cast<long long>(z.n_seqs) * z.nkv * z.parts, grid = (units + 7) / 8 * 8 * z.blocks;
+    static_assert(lds <= 159 * 1024, "a CU's LDS");
+    if (chunk % (KT * KS) != 0 || parts > kMostParts) return EGPT_BAD_ARGUMENT;
+    const int blocks = (max_rows + 32 * RB - 1) / (32 * RB);
+    const long long units = static_cast<long long>(z.n_seqs) * nkv * parts, grid = (units + 7) / 8 * 8 * blocks;
     if (grid >= 1 << 27) return EGPT_UNSUPPORTED_SIZE;
     auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
-    if (lds > 64 * 1024) {
+    if (lds > 60 * 1024) {
         static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
         if (!raised) return EGPT_UNSUPPORTED_SIZE;
     }
-    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, q_start, block_table, static_cast<const T*>(qkv), visible, positions,
+    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, blocks, magic_of(blocks), parts, magic_of(parts), nkv,
+                                                                   magic_of(nkv), table_width, chunk, q_start, static_cast<const T*>(qkv), visible, positions,
                                                                    static_cast<const T*>(k_cache), static_cast<const T*>(v_cache), static_cast<T*>(out),
                                                                    part_o, part_ml, z);
     EGPT_CHECK_LAUNCH();
-    if (z.parts > 1) {
+    if (parts > 1) {
         const int nodes = max_rows / z.group;
-        tree_combine_kernel<T><<<dim3((nodes * z.nq + 3) / 4, z.n_seqs), 256, 0, s>>>(part_o, part_ml, q_start, q_len, kv_len, nodes, z.parts, z.n_tokens, z.nq, z.hd,
-                                                                                 z.chunk, magic_of(z.chunk), magic_of(z.nq), static_cast<T*>(out));
+        tree_combine_kernel<T><<<dim3((nodes * z.nq + 3) / 4, z.n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, chunk, magic_of(chunk), z.nq,
+                                                                                 magic_of(z.nq), nodes, parts, z.n_tokens, z.hd, static_cast<T*>(out));
         EGPT_CHECK_LAUNCH();
     }
     return EGPT_OK;
@@ -655,12 +700,11 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
         return EGPT_UNSUPPORTED_SIZE;
     if (n_tokens == 0 || max_q_len == 0) return EGPT_OK;
     const int group = nq / nkv;
-    const TreeSizes z{table_width, n_pages, page_size, nq, nkv, hd, group, n_seqs, parts, chunk, 1, window, n_tokens,
-                      magic_of(parts), magic_of(nkv), 0u, magic_of(group), magic_of(page_size), magic_of(chunk), scale};
+    const TreeSizes z{n_pages, page_size, nq, hd, group, n_seqs, window, n_tokens, magic_of(group), magic_of(page_size), magic_of(chunk), scale};
     const int max_rows = max_q_len * group;
 #define EGPT_TREE(...) \
-    return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, positions, z, max_rows, \
-                                    static_cast<hipStream_t>(stream))
+    return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, table_width, q_start, q_len, kv_len, visible, positions, z, nkv, parts, \
+                                    chunk, max_rows, static_cast<hipStream_t>(stream))
     // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS)
     if (dtype == 1 && hd <= 64) {
         if (shape == 1) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);
