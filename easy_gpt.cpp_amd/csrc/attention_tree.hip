@@ -175,8 +175,8 @@ __device__ __forceinline__ void load_1k(r_i32x4 resource, int offset, int more, 
 }
 #pragma clang diagnostic pop
 struct TreeSizes {
-    int n_pages, page_size, nq, hd, group, n_seqs, window, n_tokens;
-    unsigned magic_group, magic_page, magic_chunk;
+    int n_pages, page_size, nq, hd, window, n_tokens;
+    unsigned magic_group, magic_page;
     float scale;
 };
 
@@ -186,11 +186,59 @@ constexpr int tree_lds() {
     return stages > join ? stages : join;
 }
 
+// Which request's work a workgroup has: the requests' works lie one after the other, request b has work_of(q_len[b], kv_len[b]) of them.  Workgroups go to the eight
+// dies in turn, so those of a die take works that follow each other: blocks of rows that read the same keys are on one die.  As many workgroups as works, not
+// as the most of any request for each: workgroups without work, in a pattern, leave the same compute units idle (64 requests of 1 to 32 nodes
+// behind 128 to 4,000 tokens: 154 of 256 busy).  64 requests at a time, by a sum over the lanes.  False: nobody's.
+struct TreeWork {
+    int request, index, n, kv;
+};
+template <class F>
+__device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, int n_seqs, F work_of, TreeWork& found) {
+    const int lane = threadIdx.x % kWave;
+    auto upto_of = [&](int v) {
+        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);                // row_shr:1, 2, 4, 8: the sum within a row
+        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);               // row_bcast:15 and 31: the rows before it
+        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+        return v;
+    };
+    int n = lane < n_seqs ? q_len[lane] : 0, kv = lane < n_seqs ? kv_len[lane] : 0;
+    int work = work_of(n, kv), upto = upto_of(work), total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    for (int s0 = kWave; s0 < n_seqs; s0 += kWave) {
+        const int i = s0 + lane;
+        total += __builtin_amdgcn_readlane(upto_of(i < n_seqs ? work_of(q_len[i], kv_len[i]) : 0), kWave - 1);
+    }
+    const int each = (total + 7) / 8;
+    int index = static_cast<int>(blockIdx.x % 8) * each + static_cast<int>(blockIdx.x / 8);
+    if (static_cast<int>(blockIdx.x / 8) >= each || index >= total) return false;
+    for (int s0 = 0;;) {
+        const unsigned long long behind = __ballot(upto > index);
+        if (behind != 0) {
+            const int at = __builtin_ctzll(behind);
+            found.request = s0 + at;
+            found.index = index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(work, at));
+            found.n = __builtin_amdgcn_readlane(n, at);
+            found.kv = __builtin_amdgcn_readlane(kv, at);
+            return true;
+        }
+        index -= __builtin_amdgcn_readlane(upto, kWave - 1);
+        s0 += kWave;
+        const int i = s0 + lane;
+        n = i < n_seqs ? q_len[i] : 0;
+        kv = i < n_seqs ? kv_len[i] : 0;
+        work = work_of(n, kv);
+        upto = upto_of(work);
+    }
+}
+
 // (the first 14 words of the arguments arrive with the wavefronts: all that the first trip to memory needs)
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1) void tree_attention_kernel(
-    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int blocks, unsigned magic_blocks,
-    int parts, unsigned magic_parts, int nkv, unsigned magic_nkv, int table_width, int chunk, const int32_t* __restrict__ q_start,
+    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int n_seqs, int nkv, int parts,
+    int chunk, unsigned magic_chunk, int group, int max_q_len, int table_width, const int32_t* __restrict__ q_start,
     const T* __restrict__ qkv, const long long* __restrict__ visible, const int32_t* __restrict__ positions, const T* __restrict__ k_cache,
     const T* __restrict__ v_cache, T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml, TreeSizes z) {
     constexpr int SZ = sizeof(T);
@@ -206,15 +254,15 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 32, lh = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), rb = wave % RB, ksi = wave / RB;
 
-    // Which part of which request and kv head, and which block of its rows.  Workgroups go to the eight dies in turn: the blocks of rows that read the same
-    // keys follow each other on one of them.
-    const int slot = blockIdx.x / 8;
-    const int unit0 = divided(slot, blocks, magic_blocks);
-    const int block = slot - unit0 * blocks, unit = unit0 * 8 + blockIdx.x % 8;
-    const int pair = divided(unit, parts, magic_parts), part = unit - pair * parts;
-    const int b = divided(pair, nkv, magic_nkv), kvh = pair - b * nkv;
-    if (b >= z.n_seqs) return;
-    const int n = q_len[b], kv_all = kv_len[b], qs = q_start[b];
+    // which part of which request and kv head, and which block of its rows
+    auto blocks_of = [&](int n_) { return (min(max(n_, 0), max_q_len) * group + 32 * RB - 1) / (32 * RB); };
+    auto parts_of = [&](int kv_) { return min(divided(max(kv_, 1) - 1, chunk, magic_chunk) + 1, parts); };
+    TreeWork work;
+    if (!find_work(q_len, kv_len, n_seqs, [&](int n_, int kv_) { return blocks_of(n_) * parts_of(kv_) * nkv; }, work)) return;
+    const int b = work.request, n = work.n, kv_all = work.kv;
+    const int blocks = blocks_of(n), n_parts = parts_of(kv_all);
+    const int unit = work.index / blocks, block = work.index - unit * blocks, kvh = unit / n_parts, part = unit - kvh * n_parts;
+    const int qs = q_start[b];
     const int from = part * chunk;
     // The pages of 64 groups of keys, a lane each, asked for before it is known how many keys there are; the next 64 while these are walked.
     const int32_t* const table = block_table + static_cast<size_t>(b) * table_width;
@@ -227,11 +275,8 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
         return Places{page >= z.n_pages ? -1 : page, key - at * z.page_size};
     };
     Places here = places_from(from);
-    const int rows = n * z.group, row0 = block * 32 * RB;
-    if (row0 >= rows) return;
+    const int rows = n * group, row0 = block * 32 * RB;
     const int before = kv_all - n, kv = min(kv_all, table_width * z.page_size);
-    const int n_parts = min(divided(max(kv_all, 1) - 1, chunk, z.magic_chunk) + 1, parts);
-    if (part >= n_parts) return;
     const int to = min(kv, from + chunk);
     const int groups = to > from ? (to - from + kGroup - 1) / kGroup : 0;
 
@@ -273,9 +318,9 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 
     // this lane's row
     const int r = row0 + rb * 32 + lr;
-    const int node_at = divided(r, z.group, z.magic_group);
+    const int node_at = divided(r, group, z.magic_group);
     const bool valid = r < rows && qs >= 0 && qs + node_at < z.n_tokens;
-    const int node = valid ? node_at : 0, head = kvh * z.group + (valid ? r - node * z.group : 0);
+    const int node = valid ? node_at : 0, head = kvh * group + (valid ? r - node * group : 0);
     const int token = qs + node;
     // the first round: with a window the one that has the first key that any row of the workgroup sees
     int lo = valid ? 0 : 0x7fffffff, first_round = 0, all_see = 0;       // all_see: from which key on all rows see everything before the tree
@@ -366,7 +411,8 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             l_run = l_run * alpha + (sees && lh == 0 ? w : 0.f);             // (the halves' sums are added up in the end)
             const char* const values = tile + HALF + key / kGroup * HD * kGroup * SZ;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DB; ++d) {
+                asm volatile("" ::: "memory");                                // (not all of them at once)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int feature = d * 32 + e / 4 * 8 + lh * 4 + e % 4, in = key % kGroup;
@@ -376,6 +422,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
                     const float scaled = acc[d][e] * alpha;
                     acc[d][e] = sees ? fmaf(w, v, scaled) : scaled;
                 }
+            }
         }
     };
     // A tile.  MASKED: its scores are compared with what the row sees.
@@ -629,27 +676,28 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __rest
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
                        int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
-                       const int32_t* positions, const TreeSizes& z, int nkv, int parts, int chunk, int max_rows, hipStream_t s) {
+                       const int32_t* positions, const TreeSizes& z, int n_seqs, int nkv, int group, int max_q_len, int parts, int chunk, hipStream_t s) {
     constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS>();
     static_assert(lds <= 159 * 1024, "a CU's LDS");
     if (chunk % (KT * KS) != 0 || parts > kMostParts) return EGPT_BAD_ARGUMENT;
-    const int blocks = (max_rows + 32 * RB - 1) / (32 * RB);
-    const long long units = static_cast<long long>(z.n_seqs) * nkv * parts, grid = (units + 7) / 8 * 8 * blocks;
+    // (no more works than this: blocks of rows of all tokens and one begun per request, and the most blocks of a request times the requests)
+    const long long rows = static_cast<long long>(z.n_tokens) * group, blocks = (max_q_len * group + 32 * RB - 1) / (32 * RB);
+    const long long works = (rows / (32 * RB) + n_seqs < blocks * n_seqs ? rows / (32 * RB) + n_seqs : blocks * n_seqs) * nkv * parts;
+    const long long grid = (works + 7) / 8 * 8;
     if (grid >= 1 << 27) return EGPT_UNSUPPORTED_SIZE;
     auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
     if (lds > 60 * 1024) {
         static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
         if (!raised) return EGPT_UNSUPPORTED_SIZE;
     }
-    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, blocks, magic_of(blocks), parts, magic_of(parts), nkv,
-                                                                   magic_of(nkv), table_width, chunk, q_start, static_cast<const T*>(qkv), visible, positions,
+    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, chunk, magic_of(chunk), group, max_q_len,
+                                                                   table_width, q_start, static_cast<const T*>(qkv), visible, positions,
                                                                    static_cast<const T*>(k_cache), static_cast<const T*>(v_cache), static_cast<T*>(out),
                                                                    part_o, part_ml, z);
     EGPT_CHECK_LAUNCH();
     if (parts > 1) {
-        const int nodes = max_rows / z.group;
-        tree_combine_kernel<T><<<dim3((nodes * z.nq + 3) / 4, z.n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, chunk, magic_of(chunk), z.nq,
-                                                                                 magic_of(z.nq), nodes, parts, z.n_tokens, z.hd, static_cast<T*>(out));
+        tree_combine_kernel<T><<<dim3((max_q_len * z.nq + 3) / 4, n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, chunk, magic_of(chunk), z.nq,
+                                                                                 magic_of(z.nq), max_q_len, parts, z.n_tokens, z.hd, static_cast<T*>(out));
         EGPT_CHECK_LAUNCH();
     }
     return EGPT_OK;
@@ -682,7 +730,7 @@ extern "C" int egpt_tree_attention_generic(const void* qkv, void* out, const voi
     return EGPT_OK;
 }
 
-// shape: blocks of 32 rows that a workgroup takes, 1, 2, 4 or 8.
+// shape: 10 * (blocks of 32 rows that a workgroup takes) + wavefronts that share a block's keys.
 extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache,
                                    const int32_t* block_table, int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len,
                                    const int32_t* kv_len, const long long* visible, const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv,
@@ -700,34 +748,29 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
         return EGPT_UNSUPPORTED_SIZE;
     if (n_tokens == 0 || max_q_len == 0) return EGPT_OK;
     const int group = nq / nkv;
-    const TreeSizes z{n_pages, page_size, nq, hd, group, n_seqs, window, n_tokens, magic_of(group), magic_of(page_size), magic_of(chunk), scale};
-    const int max_rows = max_q_len * group;
+    const TreeSizes z{n_pages, page_size, nq, hd, window, n_tokens, magic_of(group), magic_of(page_size), scale};
 #define EGPT_TREE(...) \
-    return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, table_width, q_start, q_len, kv_len, visible, positions, z, nkv, parts, \
-                                    chunk, max_rows, static_cast<hipStream_t>(stream))
+    return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, table_width, q_start, q_len, kv_len, visible, positions, z, n_seqs, nkv, \
+                                    group, max_q_len, parts, chunk, static_cast<hipStream_t>(stream))
     // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS)
     if (dtype == 1 && hd <= 64) {
-        if (shape == 1) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);
-        if (shape == 2) EGPT_TREE(bf16_t, 64, 2, 2, 64, 2);
-        if (shape == 4) EGPT_TREE(bf16_t, 64, 4, 1, 64, 3);
-        if (shape == 8) EGPT_TREE(bf16_t, 64, 8, 1, 64, 3);
+        if (shape == 14) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);
+        if (shape == 22) EGPT_TREE(bf16_t, 64, 2, 2, 64, 2);
+        if (shape == 41) EGPT_TREE(bf16_t, 64, 4, 1, 64, 2);
     } else if (dtype == 1 && hd <= 128) {
-        if (shape == 1) EGPT_TREE(bf16_t, 128, 1, 4, 32, 2);
-        if (shape == 2) EGPT_TREE(bf16_t, 128, 2, 2, 64, 2);
-        if (shape == 4) EGPT_TREE(bf16_t, 128, 4, 1, 64, 2);
-        if (shape == 8) EGPT_TREE(bf16_t, 128, 8, 1, 64, 3);
+        if (shape == 22) EGPT_TREE(bf16_t, 128, 2, 2, 32, 2);
+        if (shape == 81) EGPT_TREE(bf16_t, 128, 8, 1, 64, 3);
     } else if (dtype == 1) {
-        if (shape == 1) EGPT_TREE(bf16_t, 256, 1, 2, 32, 2);
-        if (shape == 4) EGPT_TREE(bf16_t, 256, 4, 1, 32, 3);
+        if (shape == 12) EGPT_TREE(bf16_t, 256, 1, 2, 32, 2);
+        if (shape == 41) EGPT_TREE(bf16_t, 256, 4, 1, 32, 3);
     } else if (hd <= 64) {
-        if (shape == 1) EGPT_TREE(float, 64, 1, 4, 32, 2);
-        if (shape == 2) EGPT_TREE(float, 64, 2, 2, 32, 2);
-        if (shape == 4) EGPT_TREE(float, 64, 4, 1, 32, 3);
+        if (shape == 14) EGPT_TREE(float, 64, 1, 4, 32, 2);
+        if (shape == 22) EGPT_TREE(float, 64, 2, 2, 32, 2);
     } else if (hd <= 128) {
-        if (shape == 1) EGPT_TREE(float, 128, 1, 2, 32, 2);
-        if (shape == 4) EGPT_TREE(float, 128, 4, 1, 32, 3);
-    } else {
-        if (shape == 4) EGPT_TREE(float, 256, 4, 1, 32, 2);
+        if (shape == 22) EGPT_TREE(float, 128, 2, 2, 32, 2);
+        if (shape == 41) EGPT_TREE(float, 128, 4, 1, 32, 2);
+    } else if (shape == 41) {
+        EGPT_TREE(float, 256, 4, 1, 32, 2);
     }
 #undef EGPT_TREE
     return EGPT_BAD_ARGUMENT;

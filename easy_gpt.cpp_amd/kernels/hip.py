@@ -2239,7 +2239,7 @@ class HipKernels(KernelBackend):
         if t == 0 or b == 0:
             return
         if hd * qkv.element_size() % 16 == 0 and page_size % 16 == 0 and not (qkv.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
-            shape, parts, chunk = self._tree_shape(b, nkv, nq // nkv, hd, dt, max_q_len, max_kv_len)
+            shape, parts, chunk = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 256) * 256)
             part_o = part_ml = None
             if parts > 1:
                 part_o = torch.empty((parts, t, nq, hd), dtype=_F32, device=qkv.device)
@@ -2253,23 +2253,44 @@ class HipKernels(KernelBackend):
                   width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
                   positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), dt, self._stream())
 
-    @staticmethod
+    # The matrix-core kernel for trees by type (0 float32) and head size: its shapes (10 * blocks of 32 rows to a workgroup + wavefronts that share a
+    # block's keys), keys of a round, workgroups that a CU holds, and a fit of what was measured (50 sizes of 1 to 64 requests, 1 to 64 nodes,
+    # 128 to 32,000 tokens before them, in up to 64 parts): microseconds before the first round, of a round with one workgroup to a CU and with as
+    # many as it holds.  (By the fit's choice 3 % slower than the best of what was measured; 64 requests of 1 to 32 nodes behind 128 to 4,000 tokens 17 %,
+    # whose sums it cannot know.)
+    _tree_shapes = {
+        (1, 64): ((14, 128, 2, 5.95, 0.77, 1.28), (22, 128, 2, 5.46, 1.05, 1.68), (41, 64, 3, 5.2, 0.93, 1.15)),
+        (1, 128): ((22, 64, 2, 6.74, 1.03, 1.43), (81, 64, 1, 6.24, 1.96, 1.96)),
+        (1, 256): ((12, 64, 1, 6.95, 2.25, 2.25), (41, 32, 1, 5.7, 2.08, 2.08)),
+        (0, 64): ((14, 128, 1, 5.12, 3.37, 3.37), (22, 64, 2, 6.39, 2.4, 4.75)),
+        (0, 128): ((22, 64, 1, 7.4, 4.86, 4.86), (41, 32, 2, 6.85, 4.14, 11.0)),
+        (0, 256): ((41, 32, 1, 7.0, 8.0, 8.0),),
+    }
+
+    @classmethod
     @functools.lru_cache(maxsize=4096)
-    def _tree_shape(b, nkv, group, hd, dt, max_q_len, max_kv_len) -> tuple[int, int, int]:
-        """(blocks of 32 rows to a workgroup, parts of the keys at most, keys of a part) of the matrix-core kernel."""
-        rows = max_q_len * group
-        shape = 1 if rows <= 32 else 2 if rows <= 64 else 4 if rows <= 128 else 8
-        if dt == 0 or hd > 128:
-            shape = min(shape, 4)
-            if shape == 2 and hd > (64 if dt == 0 else 128):
-                shape = 4
-            if shape < 4 and dt == 0 and hd > 128:
-                shape = 4
-        units = b * nkv * -(-rows // (32 * shape))
-        most = -(-max_kv_len // 128)
-        parts = max(1, min(512 // units, most, 64), -(-max_kv_len // 8192))
-        chunk = max(1, -(-most // parts)) * 128
-        return shape, max(1, -(-max_kv_len // chunk)), chunk
+    def _tree_shape(cls, b, t, nkv, group, hd, dt, max_q_len, max_kv_len) -> tuple[int, int, int]:
+        """(shape, parts of a request's keys at most, keys of a part) of the matrix-core kernel for trees: the cheapest by the fit.  The joining
+        kernel costs 2.9 us and 0.25 for a megabyte of the parts' results."""
+        best = None
+        for shape, keys, held, launch, alone, full in cls._tree_shapes[dt, 64 if hd <= 64 else 128 if hd <= 128 else 256]:
+            rows = 32 * (shape // 10)
+            blocks = min(-(-max_q_len * group // rows) * b, t * group // rows + b) * nkv
+            rounds = last = -(-max_kv_len // keys)
+            for wanted in (1, 2, 3, 4, 6, 8, 11, 16, 22, 32, 48, 64):
+                per = max(-(-rounds // wanted), 1)                   # rounds of a part
+                parts = -(-rounds // per)
+                if parts == last and wanted > 1:
+                    continue
+                last = parts
+                works = blocks * parts
+                turns = max(1, -(-works // (256 * held)))
+                us = launch + turns * per * (alone + (full - alone) * min(1.0, max(0.0, works / turns / 256 - 1) / max(held - 1, 1))) + (turns - 1) * 1.5
+                if parts > 1:
+                    us += 2.9 + 0.25e-6 * parts * t * group * nkv * hd * 8
+                if best is None or us < best[0]:
+                    best = us, shape, parts, per * keys
+        return best[1:]
 
     def accept_drafts(self, tokens, parents, sampled, q_start, q_len):
         t, b = tokens.shape[0], q_len.shape[0]
