@@ -162,9 +162,9 @@ class HipKernels(KernelBackend):
 
     # ------------------------------------------------------------------ helpers
     def _stream(self):
-        """The stream to launch on: torch's current one.  Asking torch costs several microseconds, and a step
-        launches a couple of hundred kernels, so a model's forward pass asks once (`pinned_stream`)."""
-        return self._pinned if self._pinned is not None else torch.cuda.current_stream().cuda_stream
+        """The stream to launch on: torch's current one.  A step launches a couple of hundred kernels, so a model's forward
+        pass asks once (`pinned_stream`).  (The handle alone: an object for it, torch.cuda.current_stream(), costs 4 us.)"""
+        return self._pinned if self._pinned is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
     def pinned_stream(self):
         """Context manager: within it every launch goes to the stream that is current on entry.  The caller
@@ -2179,13 +2179,9 @@ class HipKernels(KernelBackend):
     def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None):
         r, v = logits.shape
         self._need(logits, "logits", _F32)
-        self._need(temperature, "temperature", _F32, (r,))
-        self._need(top_k, "top_k", _I32, (r,))
-        self._need(top_p, "top_p", _F32, (r,))
-        self._need(uniform, "uniform", _F32, (r,))
-        self._need(out, "out", _I32, (r,))
-        if min_p is not None:
-            self._need(min_p, "min_p", _F32, (r,))
+        device = logits.get_device()
+        self._lists(device, _F32, r, (temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform"), *(() if min_p is None else ((min_p, "min_p"),)))
+        self._lists(device, _I32, r, (top_k, "top_k"), (out, "out"))
         if v >= 8192:
             # a wide vocabulary: the row-wide passes by many workgroups, the selection on the tokens that are left
             space = torch.empty(int(self.lib.egpt_sample_workspace(r, v)), dtype=torch.uint8, device=logits.device)
@@ -2197,61 +2193,72 @@ class HipKernels(KernelBackend):
                   uniform.data_ptr(), out.data_ptr(), weights.data_ptr(), r, v, self._stream())
 
     # ------------------------------------------------------------------ drafted tokens
-    @staticmethod
-    def _here(t: torch.Tensor, *others) -> None:
-        """These operators launch on the current device's stream, so that is where their operands have to be."""
-        device = t.device
-        for o in others:
-            if o is not None and o.device != device:
-                raise ValueError(f"operands lie on {device} and on {o.device}")
-        if device.index != torch.cuda.current_device():
-            raise ValueError(f"operands lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    # (Calls whose kernels take a few microseconds: what is usual is told by a few cheap questions, the rest is left to the careful ones.)
+    def _here(self, t, name, dtype=None, shape=None) -> None:
+        """`_need`, and the operand lies on the current device, on whose stream the launch goes."""
+        self._need(t, name, dtype, shape)
+        if t.get_device() != torch._C._cuda_getDevice():
+            raise ValueError(f"{name} lies on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+    def _lists(self, device: int, dtype, n: int, *named) -> None:
+        """Tensors of n numbers each on that device."""
+        for t, name in named:
+            if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
+                self._here(t, name, dtype, (n,))
+
+    def _table(self, device: int, t, name: str) -> tuple[int, int]:
+        """The sizes of an int32 tensor [requests, ...] on that device."""
+        if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is _I32 and t.is_contiguous()):
+            self._here(t, name, _I32)
+        if t.dim() != 2:
+            raise ValueError(f"{name} must be [requests, ...], got {tuple(t.shape)}")
+        return t.shape
 
     def tree_attention(self, qkv, out, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, nq, nkv, hd, page_size, scale,
                        max_q_len, max_kv_len, window=0, positions=None):
-        t = qkv.shape[0]
         if nkv < 1 or nq < 1 or nq % nkv:
             raise ValueError(f"the number of query heads ({nq}) must be a multiple of that of key heads ({nkv})")
         if not 1 <= hd <= self.max_head_dim:
             raise ValueError(f"head size {hd} is not supported by the attention kernels (1 to {self.max_head_dim})")
-        if max_q_len > self.max_tree_nodes:
+        if not 0 <= max_q_len <= self.max_tree_nodes:
             raise ValueError(f"a request's tree has at most {self.max_tree_nodes} nodes, not {max_q_len}")
         if window < 0:
             raise ValueError("the window must be >= 0")
-        dt = self._act(qkv, "qkv")
-        self._need(qkv, "qkv", None, (t, (nq + 2 * nkv) * hd))
-        self._need(out, "out", qkv.dtype, (t, nq * hd))
-        self._caches(k_cache, v_cache, qkv.dtype, nkv, page_size, hd)
-        self._need(block_table, "block_table", _I32)
-        if block_table.dim() != 2:
-            raise ValueError(f"block_table must be [requests, pages of the longest], got {tuple(block_table.shape)}")
-        b, width = block_table.shape
-        for name, v in (("q_start", q_start), ("q_len", q_len), ("kv_len", kv_len)):
-            self._need(v, name, _I32, (b,))
-        self._need(visible, "visible", _I64, (t,))
+        self._here(qkv, "qkv")
+        if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * hd:
+            raise ValueError(f"qkv must be [tokens, {(nq + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
+        dt, dtype, device, t = self._act(qkv, "qkv"), qkv.dtype, qkv.get_device(), qkv.shape[0]
+        self._here(out, "out", dtype, (t, nq * hd))
+        self._here(k_cache, "k_cache", dtype)
+        self._here(v_cache, "v_cache", dtype)
+        pages = k_cache.shape[0]
+        if k_cache.shape != (pages, nkv, page_size, hd) or v_cache.shape != (pages, nkv, hd, page_size):
+            self._caches(k_cache, v_cache, dtype, nkv, page_size, hd)
+        b, width = self._table(device, block_table, "block_table")
+        self._lists(device, _I32, b, (q_start, "q_start"), (q_len, "q_len"), (kv_len, "kv_len"))
+        self._lists(device, _I64, t, (visible, "visible"))
         if window:
             if positions is None:
                 raise ValueError("a window needs the nodes' positions")
-            self._need(positions, "positions", _I32, (t,))
+            self._lists(device, _I32, t, (positions, "positions"))
         if max_kv_len > width * page_size:
             raise ValueError(f"block table of width {width} cannot hold {max_kv_len} tokens at page size {page_size}")
-        self._here(qkv, out, k_cache, v_cache, block_table, q_start, q_len, kv_len, visible, positions if window else None)
-        if t == 0 or b == 0:
+        if t == 0 or b == 0 or max_q_len == 0:
             return
-        if hd * qkv.element_size() % 16 == 0 and page_size % 16 == 0 and not (qkv.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        at_q, at_out, at_k, at_v = qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        more = (block_table.data_ptr(), width, pages, q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
+                positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window))
+        if hd * (4 if dt == 0 else 2) % 16 == 0 and page_size % 16 == 0 and not (at_q | at_out | at_k | at_v) & 15:
             shape, parts, chunk = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 256) * 256)
             part_o = part_ml = None
             if parts > 1:
-                part_o = torch.empty((parts, t, nq, hd), dtype=_F32, device=qkv.device)
-                part_ml = torch.empty((parts, t, nq, 2), dtype=_F32, device=qkv.device)
-            self._run("egpt_tree_attention", qkv.data_ptr(), out.data_ptr(), self._ptr(part_o), self._ptr(part_ml), k_cache.data_ptr(), v_cache.data_ptr(),
-                      block_table.data_ptr(), width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
-                      positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), int(max_q_len), shape, parts,
-                      chunk, dt, self._stream())
+                rows = parts * t * nq
+                part_o = torch.empty(rows * (hd + 2), dtype=_F32, device=qkv.device)
+                part_ml = part_o.data_ptr() + 4 * rows * hd
+            self._run("egpt_tree_attention", at_q, at_out, self._ptr(part_o), part_ml, at_k, at_v, *more, int(max_q_len), shape, parts, chunk, dt,
+                      self._stream())
             return
-        self._run("egpt_tree_attention_generic", qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                  width, k_cache.shape[0], q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
-                  positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window), dt, self._stream())
+        self._run("egpt_tree_attention_generic", at_q, at_out, at_k, at_v, *more, dt, self._stream())
 
     # The matrix-core kernel for trees by type (0 float32) and head size: its shapes (10 * blocks of 32 rows to a workgroup + wavefronts that share a
     # block's keys), keys of a round, workgroups that a CU holds, and a fit of what was measured (50 sizes of 1 to 64 requests, 1 to 64 nodes,
@@ -2293,38 +2300,37 @@ class HipKernels(KernelBackend):
         return best[1:]
 
     def accept_drafts(self, tokens, parents, sampled, q_start, q_len):
-        t, b = tokens.shape[0], q_len.shape[0]
-        for name, v, n in (("tokens", tokens, t), ("parents", parents, t), ("sampled", sampled, t), ("q_start", q_start, b), ("q_len", q_len, b)):
-            self._need(v, name, _I32, (n,))
-        self._here(tokens, parents, sampled, q_start, q_len)
-        path, accepted = torch.empty((2, b, self.max_tree_nodes), dtype=_I32, device=tokens.device)
-        count = torch.empty(b, dtype=_I32, device=tokens.device)
+        t, b = tokens.numel(), q_len.numel()
+        self._here(tokens, "tokens", _I32, (t,))
+        device = tokens.get_device()
+        self._lists(device, _I32, t, (parents, "parents"), (sampled, "sampled"))
+        self._lists(device, _I32, b, (q_start, "q_start"), (q_len, "q_len"))
+        on = tokens.device
+        path = torch.empty((b, self.max_tree_nodes), dtype=_I32, device=on)
+        accepted = torch.empty((b, self.max_tree_nodes), dtype=_I32, device=on)
+        count = torch.empty(b, dtype=_I32, device=on)
         self._run("egpt_accept_drafts", tokens.data_ptr(), parents.data_ptr(), sampled.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), b, t,
                   path.data_ptr(), count.data_ptr(), accepted.data_ptr(), self._stream())
         return path, count, accepted
 
     def keep_drafts(self, k_cache, v_cache, block_table, start, path, count):
-        dt = self._act(k_cache, "k_cache")
-        self._need(k_cache, "k_cache")
-        self._need(v_cache, "v_cache", k_cache.dtype)
-        if k_cache.dim() not in (4, 5) or v_cache.dim() != k_cache.dim():
+        self._here(k_cache, "k_cache")
+        dt, device = self._act(k_cache, "k_cache"), k_cache.get_device()
+        self._here(v_cache, "v_cache", k_cache.dtype)
+        keys, values = k_cache.shape, v_cache.shape
+        if len(keys) not in (4, 5) or len(values) != len(keys):
             raise ValueError("k_cache and v_cache must be [pages, ...] or [slabs, pages, ...] of pages of keys and of values")
-        pages, nkv, page_size, dk = k_cache.shape[-4:]
-        dv = v_cache.shape[-2]
-        if tuple(v_cache.shape) != (*k_cache.shape[:-2], dv, page_size):
-            raise ValueError(f"v_cache must be {(*k_cache.shape[:-2], dv, page_size)} beside keys {tuple(k_cache.shape)}, got {tuple(v_cache.shape)}")
-        self._need(block_table, "block_table", _I32)
-        self._need(path, "path", _I32)
-        if block_table.dim() != 2 or path.dim() != 2:
-            raise ValueError("block_table and path must be [requests, ...]")
-        b, width = block_table.shape
-        if path.shape[0] != b:
-            raise ValueError(f"path must have {b} rows, got {path.shape[0]}")
-        self._need(start, "start", _I32, (b,))
-        self._need(count, "count", _I32, (b,))
-        self._here(k_cache, v_cache, block_table, start, path, count)
-        if k_cache.numel() == 0 or b == 0 or width == 0 or path.shape[1] == 0:
+        pages, nkv, page_size, dk = keys[-4:]
+        dv = values[-2]
+        if values[:-2] != keys[:-2] or values[-1] != page_size:
+            raise ValueError(f"v_cache must be {(*keys[:-2], dv, page_size)} beside keys {tuple(keys)}, got {tuple(values)}")
+        b, width = self._table(device, block_table, "block_table")
+        n, path_width = self._table(device, path, "path")
+        if n != b:
+            raise ValueError(f"path must have {b} rows, got {n}")
+        self._lists(device, _I32, b, (start, "start"), (count, "count"))
+        if k_cache.numel() == 0 or b == 0 or width == 0 or path_width == 0:
             return
         self._run("egpt_keep_drafts", k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), width, start.data_ptr(), path.data_ptr(),
-                  path.shape[1], count.data_ptr(), b, k_cache.shape[0] if k_cache.dim() == 5 else 1, pages, page_size, nkv, dk, dv, dt,
+                  path_width, count.data_ptr(), b, keys[0] if len(keys) == 5 else 1, pages, page_size, nkv, dk, dv, dt,
                   self._stream())
