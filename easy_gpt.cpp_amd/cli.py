@@ -22,6 +22,7 @@ USAGE = """Usage: easy_llm [--model <dir>] [--prompt-file <path>] [--max-steps <
       --temperature <float> Sampling temperature (default: 0.8)
       --top-p <float>        Nucleus sampling cutoff in (0,1] (default: 0.95)
       --top-k <int>          Top-K sampling cutoff, 0 disables (default: 20)
+      --min-p <float>        Least probability beside the most likely token's in [0,1], 0 disables (default: 0)
       --seed <int>           RNG seed for sampling (default: 42)
       --greedy               Use greedy decoding (override sampling)
       --serve-max-active <n> Max concurrent active requests (default: 16)
@@ -40,6 +41,8 @@ USAGE = """Usage: easy_llm [--model <dir>] [--prompt-file <path>] [--max-steps <
       --prefill-chunk <n>    Largest prompt portion in one step (default: 512)
       --cache-tokens <n>     Tokens the paged cache holds (default: 65536)
       --page-size <n>        Tokens per cache page (default: 16)
+      --draft-nodes <n>      Tokens that a step checks for a decoding request, up to 64: its last one and what its own
+                             tokens say may follow (default: 0, the last one alone)
       --tune-products        Choose the library's matrix products by measurement (about a second per new shape)
   -h, --help                Show this help message
 Examples:
@@ -78,6 +81,8 @@ class CliOptions:
     page_size: int = 16
     tune_products: bool = False
     allow_unexpected_tensors: bool = False
+    min_p: float = 0.0
+    draft_nodes: int = 0
 
 
 class CliError(ValueError):
@@ -131,6 +136,14 @@ def parse_args(argv: list[str]) -> CliOptions:
             o.top_k = _number(int, value(arg), "top-k")
             if o.top_k < 0:
                 raise CliError("Top-k must be >= 0")
+        elif arg == "--min-p":
+            o.min_p = _number(float, value(arg), "min-p")
+            if not 0.0 <= o.min_p <= 1.0:
+                raise CliError("Min-p must be in [0, 1]")
+        elif arg == "--draft-nodes":
+            o.draft_nodes = _number(int, value(arg), "draft nodes")
+            if not 0 <= o.draft_nodes <= 64:
+                raise CliError("draft-nodes must be in [0, 64]")
         elif arg == "--seed":
             o.seed = _number(int, value(arg), "seed")
             if o.seed < 0:
@@ -252,7 +265,7 @@ def main(argv: list[str] | None = None) -> int:
     llm = LLM(o.model, dtype=o.dtype, device=o.device, cache_tokens=o.cache_tokens, page_size=o.page_size,
               max_active=o.serve_max_active, max_admit_per_step=o.serve_prefill_batch,
               max_tokens_per_step=o.max_tokens_per_step, prefill_chunk=o.prefill_chunk, tune_products=o.tune_products,
-              allow_unexpected_tensors=o.allow_unexpected_tensors)
+              allow_unexpected_tensors=o.allow_unexpected_tensors, draft_nodes=o.draft_nodes)
     last = [time.perf_counter()]
 
     def on_step(sched):
@@ -266,7 +279,7 @@ def main(argv: list[str] | None = None) -> int:
     t0 = time.perf_counter()
     requests = llm.generate_requests(
         prompts, max_new_tokens=o.max_new_tokens or 100, max_steps=None if o.max_new_tokens else o.max_steps,
-        temperature=o.temperature, top_p=o.top_p, top_k=o.top_k, greedy=o.use_greedy, seed=o.seed,
+        temperature=o.temperature, top_p=o.top_p, top_k=o.top_k, greedy=o.use_greedy, seed=o.seed, min_p=o.min_p,
         ignore_eos=o.ignore_eos, on_step=on_step,
     )
     dt = time.perf_counter() - t0

@@ -1,4 +1,5 @@
 from .context import GroupTables, StepContext
-from .engine import DTYPES, Engine, StepEntry, load_model
+from .drafting import PromptLookup
+from .engine import DTYPES, DraftEntry, Engine, StepEntry, load_model
 
-__all__ = ["DTYPES", "Engine", "GroupTables", "StepContext", "StepEntry", "load_model"]
+__all__ = ["DTYPES", "DraftEntry", "Engine", "GroupTables", "PromptLookup", "StepContext", "StepEntry", "load_model"]

@@ -29,6 +29,9 @@ class StepContext:
     single_token_requests  False when no request of the step brings exactly one token: a kernel that takes those apart
                            from the portions of prompts need not run
     spread                 of a step of decoded tokens: 0 where the longest context is within 1.4 of the mean, 1 within 2.5, 2 beyond
+    trees                  of a step of drafted tokens, by a cache group's window (0: none): int64 [T], bit m of a token's number says that it
+                           reads its request's m-th token of the step (None: tokens follow each other).  Positions are then depths
+                           in the tree behind the tokens before it; places in the cache follow each other as always
     portion_kv             a bound on kv_len over the requests that bring more than one token (None: max_kv_len)
     """
 
@@ -58,6 +61,7 @@ class StepContext:
     single_token_requests: bool = True     # False when the step is known to hold no request of exactly one token
     spread: int = 0
     portion_kv: int | None = None
+    trees: dict | None = None
 
     def cache_view(self, cache_id: int, writes: bool) -> CacheView:
         g, j = self.cache_location[cache_id]

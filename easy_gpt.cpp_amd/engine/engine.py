@@ -33,6 +33,20 @@ DTYPES = {
 
 
 @dataclass
+class DraftEntry:
+    """A request's last token and what a drafter thinks may follow it: a tree of at most 64 nodes.  Node 0 is the token that was
+    sampled last (parents[0] is -1), node i > 0 drafts tokens[i] behind node parents[i] < i."""
+
+    request_id: object
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+    @property
+    def want(self):                                         # (every node's logits)
+        return range(len(self.tokens))
+
+
+@dataclass
 class StepEntry:
     """The next tokens of one request and the places among them whose logits are wanted."""
 
@@ -132,6 +146,8 @@ class Engine:
         self._decode_plans: dict = {}
         self._row_plans: dict = {}
         self._padded_plans: dict = {}
+        self._draft_plans: dict = {}
+        self.graph_drafts = 256     # steps of at most this many drafted tokens run from a graph, which holds the logits of all of them
         self.graph_tokens = 2048    # steps of at most this many tokens run from a graph for their padded size
         self.capture_after = 1      # a shape's graph is captured right after this visit (None: never, the same kernels one by one)
         self.graph_rows = 64        # steps of at most this many tokens in all run as rows of one token each,
@@ -186,9 +202,10 @@ class Engine:
             logits = self.model.forward(ctx)
         return logits
 
-    def _check(self, entries) -> list[RequestCache]:
+    def _check(self, entries, depths=None) -> list[RequestCache]:
+        """The entries' requests.  depths: of drafted tokens, how far behind the tokens before them they stand."""
         rcs, seen = [], set()
-        for e in entries:
+        for i, e in enumerate(entries):
             if e.request_id in seen:
                 raise ValueError(f"request {e.request_id!r} appears twice in one step")
             seen.add(e.request_id)
@@ -206,9 +223,10 @@ class Engine:
             for w in e.want:
                 if not 0 <= int(w) < n:
                     raise IndexError(f"wanted place {w} of request {e.request_id!r} is outside its {n} tokens")
-            if rc.num_tokens + n > self.max_position:
+            more = n if depths is None else 1 + max(depths[i])
+            if rc.num_tokens + more > self.max_position:
                 raise ValueError(
-                    f"request {e.request_id!r} would reach {rc.num_tokens + n} tokens, "
+                    f"request {e.request_id!r} would reach {rc.num_tokens + more} tokens, "
                     f"max_position_embeddings is {self.max_position}"
                 )
             rcs.append(rc)
@@ -279,6 +297,82 @@ class Engine:
         if tokens.dtype != torch.int32 or tuple(tokens.shape) != (len(request_ids),) or tokens.device != self.device:
             raise ValueError("tokens must be int32 [number of requests] on the engine's device")
         return self._step_decode([StepEntry(rid, (0,), (0,)) for rid in request_ids], device_tokens=tokens)
+
+    # ------------------------------------------------------------------ drafted tokens
+    @property
+    def supports_drafts(self) -> bool:
+        """Whether `step_drafts` runs this model: every layer's mixer takes trees, and none keeps a state, which would be that of
+        one order of the tokens."""
+        return not self.model.state_needs and all(b.mixer is None or b.mixer.takes_trees for b in self.model.layers)
+
+    def step_drafts(self, entries: Sequence[DraftEntry], choose) -> list[list[int]]:
+        """Check drafted tokens: one step computes the logits of every node, choose(logits float32 [T, vocab]) -> int32 [T] on the device
+        says what follows each node (rows in the order of the entries and of their nodes), and every request takes the path from its root
+        along the nodes that were chosen (`accept_drafts`).  Returns each request's new tokens, what was chosen behind the nodes of the
+        path: one at least.  The path's keys and values become the request's; the other nodes leave nothing.  A token
+        is what it would be one step at a time, as far as `choose` says the same of the same logits.  Raises OutOfPages (with the
+        cache unchanged) if the nodes do not fit."""
+        from .. import kernels
+
+        entries = list(entries)
+        if not entries:
+            return []
+        if not self.supports_drafts:
+            raise RuntimeError("this model has layers that cannot check drafted tokens")
+        trees = []
+        for e in entries:
+            if len(e.tokens) == 0 or len(e.tokens) != len(e.parents):
+                raise ValueError(f"request {e.request_id!r} needs a token and a parent for every node, and one node at least")
+            windows = {g.window or 0 for g in self.cache.groups}
+            trees.append({w: kernels.draft_masks(e.parents, w) for w in windows | {0}})
+        depths = [t[0][0] for t in trees]
+        rcs = self._check(entries, depths)
+        counts = [len(e.tokens) for e in entries]
+        total = sum(counts)
+        self.cache.reserve_step(rcs, counts)
+        try:
+            if self.use_graphs and total <= self.graph_drafts:
+                plan = self._draft_plan(rcs, counts)
+                plan.fill(rcs, entries, counts, depths, trees)
+                ctx, tree = plan.ctx, plan.tree
+                logits = self._run(plan)
+            else:
+                ctx = self._build_context(rcs, entries)
+                tree = _TreeArrays(total, len(entries), [g.window or 0 for g in self.cache.groups], self.device)
+                tree.fill(rcs, entries, depths, trees)
+                ctx.positions = tree.positions
+                ctx.trees, ctx.rows_independent, ctx.max_q_len = tree.masks, False, max(2, ctx.max_q_len)
+                logits = self.model.forward(ctx)
+            chosen = choose(logits[:total])
+            if chosen.dtype != torch.int32 or tuple(chosen.shape) != (total,) or chosen.device != logits.device:
+                raise ValueError(f"choose must return int32 [{total}] where the logits are")
+            k = kernels.backend()
+            path, count, accepted = k.accept_drafts(ctx.token_ids[:total], tree.parents[:total], chosen, ctx.q_start, ctx.q_len)
+            for tensors, tables in zip(self.kv.tensors, ctx.groups):
+                k.keep_drafts(tensors["k"], tensors["v"], tables.block_table, tree.start, path, count)
+            n = len(entries)
+            taken = count[:n].tolist()
+            new = [row[:c] for row, c in zip(accepted[:n].tolist(), taken)]
+            self.cache.commit_step(rcs, taken)
+        finally:
+            self.cache.unreserve_step(rcs)                  # the nodes that were not taken; of a step that fails, all
+        return new
+
+    def _draft_plan(self, rcs, counts) -> "_DraftPlan":
+        """The graph of a step of drafted tokens goes by its padded size, as that of any step, and by bounds on a tree's nodes (powers of two from 8)
+        and on the contexts (steps of 512), by which the attention chooses its shape."""
+        t = sum(counts)
+        t_pad = -(-t // 16) * 16
+        b_pad = 2
+        while b_pad < len(rcs) + 1:
+            b_pad *= 2
+        q_bound = 8
+        while q_bound < max(*counts, t_pad - t):            # (the padding is one more request)
+            q_bound *= 2
+        widths = self._table_widths(rcs, at_least=self._pad_pages)
+        kv_bound = -(-max(rc.num_tokens + n for rc, n in zip(rcs, counts)) // 512) * 512
+        key = (t_pad, b_pad, tuple(widths), q_bound, kv_bound)
+        return self._plan(self._draft_plans, key, lambda: _DraftPlan(self, t_pad, b_pad, widths, q_bound, kv_bound))
 
     # ------------------------------------------------------------------ one token per request, from a graph
     def _step_decode(self, entries, device_tokens: torch.Tensor | None = None) -> torch.Tensor:
@@ -369,7 +463,7 @@ class Engine:
         plan.runs += 1
         if self.capture_after is not None and plan.runs >= self.capture_after:
             graph = torch.cuda.CUDAGraph()
-            plans = (self._decode_plans, self._row_plans, self._padded_plans)
+            plans = (self._decode_plans, self._row_plans, self._padded_plans, self._draft_plans)
             if self._graph_pool is None or not any(p.graph is not None for d in plans for p in d.values()):
                 # the first graph, or the first after every earlier one was dropped (their pool went with the last)
                 self._graph_pool = torch.cuda.graph_pool_handle()
@@ -544,6 +638,17 @@ class _PaddedPlan:
 
     def fill(self, rcs, entries, counts) -> int:
         """Writes the step's metadata; returns how many logits rows are wanted (the first rows of the result)."""
+        n_want = self._write(rcs, entries, counts)
+        self._upload()
+        return n_want
+
+    def _upload(self) -> None:
+        self.dev.copy_(self.host, non_blocking=True)
+        if self.copied is None:
+            self.copied = torch.cuda.Event()
+        self.copied.record()
+
+    def _write(self, rcs, entries, counts) -> int:
         if self.copied is not None:
             self.copied.synchronize()                       # the pinned mirror is free again
         t_pad, b_pad = self.t_pad, self.b_pad
@@ -592,12 +697,60 @@ class _PaddedPlan:
         ctx.q_len_host = q_len.tolist()
         ctx.kv_len_host = kv_len.tolist()
         ctx.state_slots_host = state_slots.tolist()
-        self.dev.copy_(self.host, non_blocking=True)
-        if self.copied is None:
-            self.copied = torch.cuda.Event()
-        self.copied.record()
         return len(want)
 
+
+class _TreeArrays:
+    """What a step of drafted tokens brings beside any step's metadata, one buffer on the host and one on the device: masks int64 [T] by
+    window; parents and positions int32 [T], start int32 [B], the tokens before each request's tree."""
+
+    def __init__(self, t: int, b: int, windows, device):
+        self.t, self.b = t, b
+        self.windows = sorted(set(windows) | {0})
+        n = len(self.windows)
+        self.host = torch.zeros(n * t + -(-(2 * t + b) // 2), dtype=torch.int64, pin_memory=device.type == "cuda")
+        self.dev = torch.zeros(self.host.shape, dtype=torch.int64, device=device)
+        self.np_masks, self.np_small = self.host.numpy()[: n * t].reshape(n, t), self.host.numpy()[n * t :].view(np.int32)
+        small = self.dev[n * t :].view(torch.int32)
+        self.masks = {w: self.dev[i * t : (i + 1) * t] for i, w in enumerate(self.windows)}
+        self.parents, self.positions, self.start = small[:t], small[t : 2 * t], small[2 * t : 2 * t + b]
+        self.copied = None
+
+    def fill(self, rcs, entries, depths, trees) -> None:
+        if self.copied is not None:
+            self.copied.synchronize()                       # the host's buffer is free again
+        masks, small, t, at = self.np_masks, self.np_small, self.t, 0
+        masks[:], small[:t], small[t:] = 0, -1, 0           # (rows that pad the step see nothing)
+        for i, (rc, e, depth, tree) in enumerate(zip(rcs, entries, depths, trees)):
+            n = len(e.tokens)
+            for j, w in enumerate(self.windows):
+                masks[j, at : at + n] = tree[w][1]
+            small[at : at + n] = e.parents
+            small[t + at : t + at + n] = rc.num_tokens + np.asarray(depth, dtype=np.int32)
+            small[2 * t + i] = rc.num_tokens
+            at += n
+        self.dev.copy_(self.host, non_blocking=True)
+        if self.dev.is_cuda:
+            if self.copied is None:
+                self.copied = torch.cuda.Event()
+            self.copied.record()
+
+
+class _DraftPlan(_PaddedPlan):
+    """The static buffers and the graph of a padded step of drafted tokens, which wants the logits of all of them."""
+
+    def __init__(self, engine: Engine, t_pad: int, b_pad: int, widths: list[int], q_bound: int, kv_bound: int):
+        super().__init__(engine, t_pad, b_pad, t_pad, widths)
+        self.tree = _TreeArrays(t_pad, b_pad, [g.window or 0 for g in engine.cache.groups], engine.device)
+        ctx = self.ctx
+        ctx.positions, ctx.trees, ctx.rows_independent = self.tree.positions, self.tree.masks, False
+        ctx.max_q_len, ctx.max_kv_len = q_bound, min(ctx.max_kv_len, kv_bound)
+
+    def fill(self, rcs, entries, counts, depths, trees) -> None:
+        self._write(rcs, entries, counts)
+        self.part(6)[:] = np.arange(self.t_pad, dtype=np.int32)
+        self._upload()
+        self.tree.fill(rcs, entries, depths, trees)
 
 
 class _DecodePlan:

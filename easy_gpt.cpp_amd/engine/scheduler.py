@@ -8,6 +8,10 @@ on a FIFO queue and a stack of free slots (/root/reference/src/continuous_batch_
 that is decoding contributes its last token, and what is left of the step's token budget goes to
 prompt portions in arrival order.
 
+With drafts (`SchedulerConfig.draft_nodes`) a step in which every entry decodes checks, beside each request's last token, what its
+own tokens say may follow (`engine.drafting`), and a request may gain several tokens from it; the tokens are those that it would
+have without, since the uniform number of its n-th token is the same either way.  Steps then wait for each other.
+
 Decoding runs one step ahead of the host where it can: while a decode step is on the GPU, the next one (the same
 requests, one token each) is launched behind it with its token ids taken on the device from what the sampler leaves
 there, and only then does the host wait for the first step's tokens.  So the GPU goes from step to step without waiting
@@ -28,9 +32,11 @@ import time
 from collections import deque
 from dataclasses import dataclass, field
 
+from .. import kernels
 from ..cache import NoFreeSlot
 from ..sampling import Sampler, SamplingParams
-from .engine import StepEntry
+from .drafting import PromptLookup
+from .engine import DraftEntry, StepEntry
 
 
 @dataclass
@@ -39,8 +45,11 @@ class SchedulerConfig:
     max_admit_per_step: int = 4     # the reference's --serve-prefill-batch
     max_tokens_per_step: int = 2048
     prefill_chunk: int = 512        # a request's share of a step's budget; what is left of the budget goes to portions too
+    draft_nodes: int = 0            # tokens that a step checks for a decoding request: its last one and drafted ones (0 or 1: the last one alone)
 
     def __post_init__(self):
+        if not 0 <= self.draft_nodes <= kernels.KernelBackend.max_tree_nodes:
+            raise ValueError(f"draft_nodes must be in [0, {kernels.KernelBackend.max_tree_nodes}]")
         for name in ("max_active", "max_admit_per_step", "max_tokens_per_step", "prefill_chunk"):
             if getattr(self, name) < 1:
                 raise ValueError(f"{name} must be greater than 0")
@@ -63,6 +72,7 @@ class Request:
     t_submit: float = 0.0
     t_admit: float = 0.0
     t_finish: float = 0.0
+    lookup: PromptLookup | None = None       # with drafts: the places of its runs of tokens
 
     def all_tokens(self) -> list[int]:
         return self.prompt + self.output
@@ -104,6 +114,8 @@ class Stats:
     steps: int = 0
     steps_ahead: int = 0        # decode steps launched before the tokens of the step before them were seen
     discarded: int = 0          # tokens computed for a request after its end token, and thrown away
+    drafted: int = 0            # tokens that were drafted and checked
+    accepted: int = 0           # of those, tokens that the model said as well
     prompt_tokens: int = 0
     decode_tokens: int = 0
     generated: int = 0
@@ -127,7 +139,8 @@ class Scheduler:
         self.done: list[Request] = []
         self.stats = Stats()
         self._serial = 0
-        self.lookahead = bool(getattr(engine, "supports_lookahead", False))
+        self.drafts = self.config.draft_nodes > 1 and bool(getattr(engine, "supports_drafts", False))
+        self.lookahead = bool(getattr(engine, "supports_lookahead", False)) and not self.drafts
         self._ahead: _Launched | None = None      # the step after the one being waited for, already launched
         self._last_end = 0.0                      # when the last step's tokens were there
 
@@ -379,6 +392,91 @@ class Scheduler:
         self.stats.steps_ahead += 1
         return self._launched(nxt, logits, t0, 1)
 
+    # ------------------------------------------------------------------ drafted tokens
+    def _draft(self, entries: list[PlannedEntry]) -> list[DraftEntry] | None:
+        """What the requests' own tokens say may follow, for a step in which every entry decodes: within the step's budget, the pages that are
+        free and the tokens that each request may still have.  None: nothing is drafted."""
+        if any(e.count != 1 or not e.samples or not e.request.output for e in entries):
+            return None
+        budget = self.config.max_tokens_per_step - len(entries)
+        requests, pages = self.cache.requests, self.cache.pages_needed
+        free = [pool.free_count for pool in self.cache.pools]            # what is left when every request has its last token's place
+        for e in entries:
+            free = [f - n for f, n in zip(free, pages(requests[e.request.request_id], 1))]
+        drafts = []
+        for e in entries:
+            r = e.request
+            if r.lookup is None:
+                r.lookup = PromptLookup()
+            known = len(r.lookup.tokens)
+            r.lookup.extend(r.tokens(known, len(r.prompt) + len(r.output) - known))
+            # (the last token of a request is never stored, and none beyond its limits is asked for)
+            depth = min(r.max_new_tokens - len(r.output) - 1, self.engine.max_position - len(r.prompt) - len(r.output))
+            nodes = min(self.config.draft_nodes, 1 + budget)
+            tokens, parents = r.lookup.propose(nodes, max(depth, 0)) if nodes > 1 and depth > 0 else ([r.output[-1]], [-1])
+            rc = requests[r.request_id]
+            one = pages(rc, 1)
+            while len(tokens) > 1 and any(n - o > f for n, o, f in zip(pages(rc, len(tokens)), one, free)):
+                tokens.pop()                             # (a child lies behind its parent: what is left is a tree)
+                parents.pop()
+            free = [f - n + o for f, n, o in zip(free, pages(rc, len(tokens)), one)]
+            budget -= len(tokens) - 1
+            drafts.append(DraftEntry(r.request_id, tokens, parents))
+        return drafts if any(len(d.tokens) > 1 for d in drafts) else None
+
+    def _step_drafted(self, entries: list[PlannedEntry], drafts: list[DraftEntry]) -> list[Request]:
+        """Check the drafted tokens, and give every request those that the model says as well and the one behind them."""
+        t0 = time.perf_counter()
+        params, serials, counts = [], [], []
+        for e, d in zip(entries, drafts):
+            depth, _ = kernels.draft_masks(d.parents)
+            params += [e.request.params] * len(d.tokens)
+            serials += [e.request.serial] * len(d.tokens)
+            counts += [len(e.request.output) + n for n in depth]
+        new = self.engine.step_drafts(drafts, lambda logits: self.sampler.sample_async(logits, params, serials, counts).device)
+        finished: list[Request] = []
+        for e, d, tokens in zip(entries, drafts, new):
+            r = e.request
+            r.computed += len(tokens)
+            self.stats.drafted += len(d.tokens) - 1
+            self.stats.accepted += len(tokens) - 1
+            for i, tok in enumerate(tokens):
+                self.stats.decode_tokens += 1
+                if self._take(r, int(tok), finished):
+                    self.stats.discarded += len(tokens) - 1 - i
+                    break
+        self._count_step(t0)
+        return finished
+
+    def _take(self, r: Request, tok: int, finished: list[Request]) -> bool:
+        """The request's next token; True if it ends the request."""
+        r.output.append(tok)
+        self.stats.generated += 1
+        reason = ""
+        if not r.ignore_eos and self.eos_token_id >= 0 and tok == self.eos_token_id:
+            reason = "eos"               # the end token stays in the output, as in the reference
+        elif len(r.output) >= r.max_new_tokens:
+            reason = "length"
+        elif len(r.prompt) + len(r.output) > self.engine.max_position:
+            reason = "max_position"
+        if reason:
+            self.engine.finish(r.request_id)
+            self.running.remove(r)
+            r.status, r.finish_reason, r.t_finish = "finished", reason, time.perf_counter()
+            self.stats.finished += 1
+            self.done.append(r)
+            finished.append(r)
+        return bool(reason)
+
+    def _count_step(self, t0: float) -> None:
+        self.stats.steps += 1
+        # a step launched ahead starts while the step before it is still being waited for: its time counts from
+        # that step's end, so that the steps' times add up to the time that passed
+        t_end = time.perf_counter()
+        self.stats.step_seconds += t_end - max(t0, self._last_end)
+        self._last_end = t_end
+        self.stats.pages_high_water = max(self.stats.pages_high_water, max(p.high_water for p in self.cache.pools))
+
     def step(self) -> list[Request]:
         """One step: plan it and run it (or take the one that was launched ahead), launch the step after it if that
         can be known, then wait for this step's tokens and finish what is done.  Returns the requests that finished."""
@@ -387,6 +485,9 @@ class Scheduler:
             entries = self.plan()
             if not entries:
                 return []
+            drafts = self._draft(entries) if self.drafts else None
+            if drafts is not None:
+                return self._step_drafted(entries, drafts)
             now = self._launch(entries)
         self._ahead = self._launch_ahead(now)
         finished: list[Request] = []
@@ -398,29 +499,8 @@ class Scheduler:
                     self.stats.discarded += 1           # launched ahead of the end token that finished the request
                     self.stats.decode_tokens -= 1       # (counted when it was launched)
                     continue
-                r.output.append(int(tok))
-                self.stats.generated += 1
-                reason = ""
-                if not r.ignore_eos and self.eos_token_id >= 0 and tok == self.eos_token_id:
-                    reason = "eos"               # the end token stays in the output, as in the reference
-                elif len(r.output) >= r.max_new_tokens:
-                    reason = "length"
-                elif len(r.prompt) + len(r.output) > self.engine.max_position:
-                    reason = "max_position"
-                if reason:
-                    self.engine.finish(r.request_id)
-                    self.running.remove(r)
-                    r.status, r.finish_reason, r.t_finish = "finished", reason, time.perf_counter()
-                    self.stats.finished += 1
-                    self.done.append(r)
-                    finished.append(r)
-        self.stats.steps += 1
-        # a step launched ahead starts while the step before it is still being waited for: its time counts from
-        # that step's end, so that the steps' times add up to the time that passed
-        t_end = time.perf_counter()
-        self.stats.step_seconds += t_end - max(now.t0, self._last_end)
-        self._last_end = t_end
-        self.stats.pages_high_water = max(self.stats.pages_high_water, max(p.high_water for p in self.cache.pools))
+                self._take(r, int(tok), finished)
+        self._count_step(now.t0)
         return finished
 
     def run(self, on_step=None) -> list[Request]:

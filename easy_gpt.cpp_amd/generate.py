@@ -42,12 +42,17 @@ class LLM:
         prefill_chunk: int = 512,
         tune_products: bool = False,
         allow_unexpected_tensors: bool = False,
+        draft_nodes: int = 0,
     ):
+        """draft_nodes: tokens that a step checks for a decoding request, its last one and what its own tokens say may follow
+        (`engine.PromptLookup`); up to 64, 0 or 1: the last one alone."""
         self.engine = Engine.from_dir(model_dir, dtype=dtype, device=device, page_size=page_size,
                                       max_tokens=cache_tokens, max_requests=max_active, tune_products=tune_products,
                                       allow_unexpected_tensors=allow_unexpected_tensors)
         self.config = SchedulerConfig(max_active=max_active, max_admit_per_step=max_admit_per_step,
-                                      max_tokens_per_step=max_tokens_per_step, prefill_chunk=prefill_chunk)
+                                      max_tokens_per_step=max_tokens_per_step, prefill_chunk=prefill_chunk, draft_nodes=draft_nodes)
+        if draft_nodes > 1 and not self.engine.supports_drafts:
+            raise ValueError("this model has layers that cannot check drafted tokens (draft_nodes)")
         self.eos_token_id = self.engine.model.spec.eos_token_id
         self.last_stats = None
         self.last_requests: list[Request] = []
@@ -64,13 +69,14 @@ class LLM:
         ignore_eos: bool = False,
         max_steps: int | None = None,
         on_step=None,
+        min_p: float = 0.0,
     ) -> list[Request]:
         """One Request per prompt, in the order of the prompts, each with its `output`, `status` ("finished" or
         "failed") and `finish_reason`: a request that fails does not take the others with it.  `max_steps`, if
         given, is the reference's --max-steps: a cap on a request's total length, giving
         max(1, max_steps - len(prompt) + 1) new tokens
         (/root/reference/src/continuous_batch_server.cpp:313)."""
-        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, greedy=greedy, seed=seed)
+        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, greedy=greedy, seed=seed, min_p=min_p)
         sched = Scheduler(self.engine, self.config, eos_token_id=self.eos_token_id)
         reqs = []
         for i, p in enumerate(prompts):
@@ -93,6 +99,6 @@ class LLM:
 def generate(model_dir: str, prompts, dtype: str = "bfloat16", device: str = "cuda:0", **options) -> list[list[int]]:
     """One call: load `model_dir`, generate for `prompts` (lists of token ids)."""
     llm_keys = {"cache_tokens", "page_size", "max_active", "max_admit_per_step", "max_tokens_per_step",
-                "prefill_chunk", "tune_products", "allow_unexpected_tensors"}
+                "prefill_chunk", "tune_products", "allow_unexpected_tensors", "draft_nodes"}
     llm_opts = {k: options.pop(k) for k in list(options) if k in llm_keys}
     return LLM(model_dir, dtype=dtype, device=device, **llm_opts).generate(prompts, **options)

@@ -24,6 +24,7 @@ from .spec import ParamSpec, PartSpec
 class GQAttention(Mixer):
     graph_safe = True
     takes_pending_norm = True
+    takes_trees = True
 
     def __init__(
         self,
@@ -214,6 +215,13 @@ class GQAttention(Mixer):
 
     def _attention(self, k, qkv, ctx, cache, attn, want_parts, ranges):
         """Attention over the cache.  If the kernel splits the keys, the output projection combines the parts."""
+        trees = getattr(ctx, "trees", None)
+        if trees is not None:
+            window = self.window or 0
+            k.tree_attention(qkv, attn, cache.k, cache.v, cache.block_table, ctx.q_start, ctx.q_len, ctx.kv_len, trees[window], self.n_heads,
+                             self.n_kv_heads, self.head_dim, cache.page_size, self.scale, ctx.max_q_len, ctx.max_kv_len, window=window,
+                             positions=ctx.positions if window else None)
+            return None
         args = dict(
             nq=self.n_heads, nkv=self.n_kv_heads, hd=self.head_dim, page_size=cache.page_size,
             scale=self.scale, window=self.window or 0, max_q_len=ctx.max_q_len, max_kv_len=ctx.max_kv_len,

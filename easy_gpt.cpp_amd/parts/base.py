@@ -231,6 +231,7 @@ class Mixer(Part):
     """
 
     takes_pending_norm = False     # True: forward may be given a PendingNorm instead of x
+    takes_trees = False            # True: forward takes a step of drafted tokens (`StepContext.trees`)
 
     def cache_need(self) -> CacheNeed | None:
         return None

@@ -4,7 +4,9 @@ Options and their meaning are the reference's (/root/reference/src/sampler.cpp:3
 defaults from /root/reference/include/cli_options.hpp:9-24): greedy (or temperature <= 0)
 takes the first maximum; otherwise probabilities are raised to 1/T (softmax(logits/T)),
 cut to the top_k most likely (0 disables), then to the smallest set whose mass reaches
-top_p (1 disables), and one uniform number picks a token from what is left.
+top_p (1 disables), and one uniform number picks a token from what is left.  min_p, which the
+reference does not have, then drops the tokens less than min_p times as likely as the most likely
+one (0 disables).
 
 The reference draws from one shared mt19937 in batch order, so a request's tokens
 depend on its neighbours.  Here the uniform number of a request's n-th token is a
@@ -28,6 +30,7 @@ class SamplingParams:
     top_k: int = 20
     greedy: bool = False
     seed: int = 42
+    min_p: float = 0.0
 
     def __post_init__(self):
         if not self.greedy and not self.temperature > 0:
@@ -38,6 +41,8 @@ class SamplingParams:
             raise ValueError("Top-k must be >= 0")
         if self.seed < 0:
             raise ValueError("Seed must be >= 0")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError("Min-p must be in [0, 1]")
 
 
 _MASK = (1 << 64) - 1
@@ -113,12 +118,15 @@ class Sampler:
             # copy is queued behind the step instead of making the host wait for it (a copy from pageable memory
             # would: with a step launched ahead, that is the step whose tokens are not needed yet)
             pinned = logits.is_cuda
-            host = torch.empty((4, r), dtype=torch.float32, pin_memory=pinned)
+            least = any(p.min_p > 0 and not p.greedy for p in params)
+            host = torch.empty((5 if least else 4, r), dtype=torch.float32, pin_memory=pinned)
             rows = host.numpy()
             rows[0] = [0.0 if p.greedy else p.temperature for p in params]
             rows[1] = [p.top_p for p in params]
             fill_uniforms(params, serials, counts, rows[2])
             rows[3].view("int32")[:] = [p.top_k for p in params]
+            if least:
+                rows[4] = [p.min_p for p in params]
             dev = host.to(logits.device, non_blocking=pinned)
-            k.sample(logits, dev[0], dev[3].view(torch.int32), dev[1], dev[2], out)
+            k.sample(logits, dev[0], dev[3].view(torch.int32), dev[1], dev[2], out, **({"min_p": dev[4]} if least else {}))
         return PendingTokens(out)
