@@ -6,97 +6,13 @@
 // kept mass.  Here the kept set is found without sorting, by radix selection on the bit patterns of the
 // weights (four passes of eight bits over the row, which stays in cache; masses are added in fixed point so
 // that no decision depends on the order of additions), and the draw walks the kept weights in index order.
-// A fourth cut that the reference does not have, min_p: of what the others keep, the tokens at least min_p times as
-// likely as the most likely one.  A weight is exp((x - max) / T), so that is a comparison with min_p itself: known before
-// the row is read, where the other thresholds have to be searched for.
 #include <mutex>
 
 #include "api.h"
 #include "common.h"
+#include "sampling.h"
 
 namespace egpt {
-
-constexpr int kSampleThreads = 1024;
-
-// Calls f(index, value) for every element of p[0..n) once, spread over the workgroup's threads (thread `tid` of
-// `n_threads`).  The body reads 16 bytes per thread and keeps eight such loads in flight: a pass over a row is a
-// chain of dependent loads otherwise, and its time is their latency, not the row's size.
-template <typename F>
-__device__ __forceinline__ void for_each_in_row(const float* __restrict__ p, int n, int tid, int n_threads, F f) {
-    const int head = min(n, static_cast<int>((4u - ((reinterpret_cast<uintptr_t>(p) >> 2) & 3u)) & 3u));
-    for (int j = tid; j < head; j += n_threads) f(j, p[j]);
-    const float4* p4 = reinterpret_cast<const float4*>(p + head);
-    const int n4 = (n - head) / 4;
-    // eight loads issued before the first value is used (the compiler does not do this by itself across calls of f
-    // that hold ballots or atomic additions)
-    constexpr int kAhead = 8;
-    int i = tid;
-    for (; i + (kAhead - 1) * n_threads < n4; i += kAhead * n_threads) {
-        float4 v[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) v[u] = p4[i + u * n_threads];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int j = head + 4 * (i + u * n_threads);
-            f(j, v[u].x);
-            f(j + 1, v[u].y);
-            f(j + 2, v[u].z);
-            f(j + 3, v[u].w);
-        }
-    }
-    for (; i < n4; i += n_threads) {
-        const float4 v = p4[i];
-        const int j = head + 4 * i;
-        f(j, v.x);
-        f(j + 1, v.y);
-        f(j + 2, v.z);
-        f(j + 3, v.w);
-    }
-    for (int j = head + 4 * n4 + tid; j < n; j += n_threads) f(j, p[j]);
-}
-
-// lowest index among equal maxima (/root/reference/src/sampler.cpp:13-20: std::max_element)
-__device__ __forceinline__ void argmax_combine(float& v, int& i, float ov, int oi) {
-    if (ov > v || (ov == v && oi < i)) {
-        v = ov;
-        i = oi;
-    }
-}
-
-// The row's best token and its value (every thread); kNoToken and -infinity where there is nothing but NaN.
-struct BestToken {
-    int index;
-    float value;
-};
-constexpr int kNoToken = 0x7fffffff;
-__device__ BestToken block_argmax(const float* __restrict__ row, int vocab, float* s_val, int* s_idx) {
-    float best = -INFINITY;
-    int best_i = kNoToken;
-    for_each_in_row(row, vocab, threadIdx.x, blockDim.x, [&](int j, float v) {
-        if (v > best || (v == best && j < best_i)) {
-            best = v;
-            best_i = j;
-        }
-    });
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) {
-        const float ov = __shfl_xor(best, o, kWave);
-        const int oi = __shfl_xor(best_i, o, kWave);
-        argmax_combine(best, best_i, ov, oi);
-    }
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    __syncthreads();
-    if (lane == 0) {
-        s_val[wave] = best;
-        s_idx[wave] = best_i;
-    }
-    __syncthreads();
-    const int n_waves = (blockDim.x + kWave - 1) / kWave;
-    best = s_val[0];
-    best_i = s_idx[0];
-    for (int w = 1; w < n_waves; ++w) argmax_combine(best, best_i, s_val[w], s_idx[w]);
-    return {best_i, best};
-}
 
 __global__ __launch_bounds__(kSampleThreads) void argmax_kernel(const float* __restrict__ logits,
                                                                 int32_t* __restrict__ out, int vocab) {
@@ -153,198 +69,6 @@ __global__ __launch_bounds__(64) void argmax_pick_kernel(const float* __restrict
     if (threadIdx.x == 0) out[blockIdx.x] = best;
 }
 
-// weight of token j: exp((x_j - max) / T), in [0, 1]
-__device__ __forceinline__ float weight_of(float x, float mx, float inv_t) { return expf((x - mx) * inv_t); }
-
-// Fixed-point image of a weight in [0, 1] (40 fractional bits): sums of these are integers, so a sum over the
-// row does not depend on the order in which threads add, and neither does any decision taken from it.
-__device__ __forceinline__ unsigned long long fixed_of(float w) {
-    return static_cast<unsigned long long>(static_cast<double>(w) * 1099511627776.0);
-}
-
-// The largest bit pattern tau with count(w >= tau) >= need (non-negative floats order like their bits): radix
-// selection, eight bits a level, histogram in LDS.  The weights of a row crowd into a few exponents, so the
-// lanes of a wavefront that hit the same bin first agree on one addition (a ballot and a population count).
-__device__ uint32_t select_by_count(const float* __restrict__ w, int vocab, unsigned int need, unsigned int* hist,
-                                    uint32_t* shared_prefix, unsigned int* shared_need) {
-    uint32_t prefix = 0u, mask = 0u;
-    const int lane = threadIdx.x % kWave;
-    int first_level = 3;
-    {
-        // The highest digit of a weight's pattern is its exponent (two exponents a bin), and the k-th largest
-        // weight is almost always within 2^-15 of the largest (1.0, digit 0x3f): count those eight bins in
-        // registers.  If the k-th weight is smaller still, the general histogram below takes over.
-        unsigned int c[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        for_each_in_row(w, vocab, threadIdx.x, blockDim.x, [&](int, float wj) {
-            const uint32_t bits = __float_as_uint(wj);
-            if (bits >= 0x38000000u) {
-                const uint32_t d = 0x3fu - (bits >> 24);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) c[i] += d == static_cast<uint32_t>(i) ? 1u : 0u;
-            }
-        });
-        for (int i = threadIdx.x; i < 8; i += blockDim.x) hist[i] = 0u;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            unsigned int v = c[i];
-#pragma unroll
-            for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-            if (lane == 0 && v) atomicAdd(&hist[i], v);          // integer sums: order does not matter
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned int cum = 0u;
-            int found = -1;
-            for (int i = 0; i < 8; ++i) {
-                if (cum + hist[i] >= need) {
-                    found = i;
-                    break;
-                }
-                cum += hist[i];
-            }
-            *shared_prefix = found >= 0 ? (0x3fu - found) << 24 : 0xffffffffu;
-            *shared_need = found >= 0 ? need - cum : need;
-        }
-        __syncthreads();
-        if (*shared_prefix != 0xffffffffu) {
-            prefix = *shared_prefix;
-            need = *shared_need;
-            mask = 255u << 24;
-            first_level = 2;
-        }
-        __syncthreads();
-    }
-    for (int level = first_level; level >= 0; --level) {
-        const int shift = 8 * level;
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0u;
-        __syncthreads();
-        for_each_in_row(w, vocab, threadIdx.x, blockDim.x, [&](int, float wj) {
-            const uint32_t bits = __float_as_uint(wj);
-            const uint32_t bin = (bits & mask) == prefix ? (bits >> shift) & 255u : 0xffffffffu;
-            unsigned long long todo = __ballot(bin != 0xffffffffu);      // over the lanes that are here
-            while (todo) {
-                const int leader = __ffsll(static_cast<long long>(todo)) - 1;
-                const uint32_t b0 = __shfl(bin, leader, kWave);
-                const unsigned long long same = __ballot(bin == b0);
-                if (lane == leader) atomicAdd(&hist[b0], static_cast<unsigned int>(__popcll(same)));
-                todo &= ~same;
-            }
-        });
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned int cum = 0u;
-            int bin = 255;
-            for (; bin > 0; --bin) {
-                if (cum + hist[bin] >= need) break;
-                cum += hist[bin];
-            }
-            *shared_prefix = prefix | (static_cast<uint32_t>(bin) << shift);
-            *shared_need = need - cum;
-        }
-        __syncthreads();
-        prefix = *shared_prefix;
-        need = *shared_need;
-        mask |= 255u << shift;
-        __syncthreads();
-    }
-    return prefix;
-}
-
-// Among the weights >= lo, the largest bit pattern tau with mass(w >= tau) >= need: the smallest set of most likely tokens whose
-// mass reaches need, ties at tau included whole.  In between, mass(w >= lo) >= need and mass(w >= hi) = above < need.  Each pass
-// divides [lo, hi): weights that crowd into a few exponents by fifteen pivots, whose masses every thread sums in registers;
-// after that by 64 bins in LDS (152,000 weights of a row that top-p alone cuts, four such passes: 540 -> 170 us a row, where
-// seven passes of pivots walked it).  Masses are fixed-point integers, whose sums depend on no order.
-__device__ uint32_t select_by_mass(const float* __restrict__ w, int vocab, uint32_t lo, uint32_t hi, unsigned long long above,
-                                   unsigned long long need, unsigned long long* sums /* [16][15] */, uint32_t* shared_lo,
-                                   uint32_t* shared_hi, unsigned long long* shared_above) {
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n_waves = blockDim.x / kWave;
-    if (lo + 1u < hi && hi == 0x3f800001u && lo < 0x38000000u) {
-        // pivots on exponent boundaries near 1.0, where the mass is
-        const uint32_t base = 0x37000000u, step = 0x01000000u;       // pivot i = base + (i + 1) * step
-        unsigned long long acc[15];
-#pragma unroll
-        for (int i = 0; i < 15; ++i) acc[i] = 0ull;
-        for_each_in_row(w, vocab, threadIdx.x, blockDim.x, [&](int, float wj) {
-            const uint32_t bits = __float_as_uint(wj);
-            if (bits > base && bits < hi && bits >= lo) {             // only these can lie at or above a pivot
-                const unsigned long long f = fixed_of(wj);
-#pragma unroll
-                for (int i = 0; i < 15; ++i) acc[i] += bits >= base + (i + 1) * step ? f : 0ull;
-            }
-        });
-#pragma unroll
-        for (int i = 0; i < 15; ++i) {
-            unsigned long long v = acc[i];
-#pragma unroll
-            for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-            if (lane == 0) sums[wave * 15 + i] = v;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t new_lo = lo, new_hi = hi;
-            unsigned long long new_above = above;
-            for (int i = 0; i < 15; ++i) {
-                const uint32_t pivot = base + (i + 1) * step;
-                if (pivot >= hi) break;
-                if (pivot <= lo) continue;
-                unsigned long long mass = above;
-                for (int wv = 0; wv < n_waves; ++wv) mass += sums[wv * 15 + i];
-                if (mass >= need) {
-                    new_lo = pivot;
-                } else {
-                    new_hi = pivot;
-                    new_above = mass;
-                    break;
-                }
-            }
-            *shared_lo = new_lo;
-            *shared_hi = new_hi;
-            *shared_above = new_above;
-        }
-        __syncthreads();
-        lo = *shared_lo;
-        hi = *shared_hi;
-        above = *shared_above;
-        __syncthreads();
-    }
-    while (lo + 1u < hi) {                           // (every pass leaves at most 1 / 32 of the range, and one pattern in the end)
-        const int width = 32 - __clz(static_cast<int>(hi - lo - 1u));
-        const int shift = width > 6 ? width - 6 : 0;
-        if (threadIdx.x < kWave) sums[threadIdx.x] = 0ull;
-        __syncthreads();
-        for_each_in_row(w, vocab, threadIdx.x, blockDim.x, [&](int, float wj) {
-            const uint32_t bits = __float_as_uint(wj);
-            if (bits >= lo && bits < hi) atomicAdd(&sums[(bits - lo) >> shift], fixed_of(wj));
-        });
-        __syncthreads();
-        if (threadIdx.x < kWave) {
-            const int bin = kWave - 1 - lane;        // from the greatest weights down
-            const unsigned long long mine = sums[bin];
-            unsigned long long incl = mine;
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const unsigned long long up = __shfl_up(incl, o, kWave);
-                if (lane >= o) incl += up;
-            }
-            const unsigned long long reached = __ballot(above + incl >= need);
-            const int holder = reached ? __ffsll(static_cast<long long>(reached)) - 1 : kWave - 1;
-            if (lane == holder) {
-                *shared_lo = lo + (static_cast<uint32_t>(bin) << shift);
-                *shared_hi = min(hi, lo + (static_cast<uint32_t>(bin + 1) << shift));
-                *shared_above = above + incl - mine;
-            }
-        }
-        __syncthreads();
-        lo = *shared_lo;
-        hi = *shared_hi;
-        above = *shared_above;
-        __syncthreads();
-    }
-    return lo;
-}
-
 // ---- wide vocabularies: the row-wide work spread over many workgroups, the selection on what is left of the row
 //
 // The selection below walks its row a dozen times with one workgroup, which for 150,000 tokens is 300 us whatever the
@@ -377,17 +101,6 @@ constexpr float kNoTopBin = -10.5f;
 // A row with top-k whose candidates follow from the shares' maxima: nothing of it underflows, and there are k maxima.
 constexpr float kLeastExponent = -80.0f;
 
-// The least weight that min_p keeps (0: min_p cuts nothing; the most likely tokens weigh 1 and stay whatever it is).
-__device__ __forceinline__ float least_of(const float* __restrict__ min_p, int r) {
-    const float m = min_p ? min_p[r] : 0.f;
-    return m > 0.f ? fminf(m, 1.0f) : 0.f;               // (a NaN cuts nothing)
-}
-// A row that min_p alone cuts, at a weight of the top bins: its bound is known without the shares' maxima, and its candidates are listed by the pass
-// that would count the others'.
-__device__ __forceinline__ bool listed_by_least(int k, float p, float least, int vocab) {
-    return !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f) && top_bin_of(__float_as_uint(least)) < kTopBins;
-}
-
 // The k-th largest of a row's kSubPieces maxima (k <= kSubPieces; 256 threads, `mine` the maximum of thread t < kSubPieces).
 __device__ float bound_of_row(float mine, int k, float* s_sub /* [kSubPieces] */, unsigned int* s_bound) {
     const int t = threadIdx.x;
@@ -416,12 +129,11 @@ __device__ float bound_of_row(float mine, int k, float* s_sub /* [kSubPieces] */
 // back.  `first`: the thread's tokens begin + t, begin + t + 256 ..., kCollectAhead of them, on their way since the kernel began.
 constexpr int kCollectAhead = 20;
 __device__ void collect_candidates(const float* __restrict__ row, int begin, int n, const float (&first)[kCollectAhead], float mx, float inv_t,
-                                   float bound_t, float least, float* __restrict__ ow, int32_t* __restrict__ oi, int* s_n /* [2], zeros */) {
-    // (expf may be off by a unit either way: 2^-18 below the bound is below every token that is not.  `least` > 0: the bound is that weight,
-    // and nobody counts by its exponent)
-    const float tight = least > 0.f ? least : expf(bound_t) * (1.0f - 3.8147e-6f);
+                                   float bound_t, float* __restrict__ ow, int32_t* __restrict__ oi, int* s_n /* [2], zeros */) {
+    // (expf may be off by a unit either way: 2^-18 below the bound is below every token that is not)
+    const float tight = expf(bound_t) * (1.0f - 3.8147e-6f);
     const uint32_t bits = __float_as_uint(tight);
-    const float loose = least == 0.f && top_bin_of(bits) < kTopBins ? __uint_as_float(bits & 0x7f800000u) : tight;
+    const float loose = top_bin_of(bits) < kTopBins ? __uint_as_float(bits & 0x7f800000u) : tight;
     const float far = bound_t - 0.75f;                       // e^-0.75 < 1/2
     auto look = [&](float x, int j) {
         const float t = exponent_of(x, mx, inv_t);
@@ -458,8 +170,7 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
                                                           int32_t* __restrict__ list_count,
                                                           float* __restrict__ cand_w, int32_t* __restrict__ cand_idx,
                                                           unsigned int* __restrict__ piece_count,
-                                                          unsigned long long* __restrict__ piece_mass, int vocab,
-                                                          const float* __restrict__ top_p, const float* __restrict__ min_p) {
+                                                          unsigned long long* __restrict__ piece_mass, int vocab) {
     __shared__ __attribute__((aligned(16))) float s_sub[kSubPieces];
     __shared__ unsigned int s_bound;
     __shared__ int s_n[2];
@@ -473,9 +184,7 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
     const int piece = (vocab + kSamplePieces - 1) / kSamplePieces;
     const int begin = min(vocab, c * piece), n = min(vocab, begin + piece) - begin;
     // everything that can be asked for is asked for at once: what follows is a chain of waits otherwise
-    const float least = least_of(min_p, r);
-    const bool by_least = least > 0.f && listed_by_least(k, top_p[r], least, vocab);
-    const bool may_list = temp > 0.f && ((by_count && k <= kSubPieces) || by_least);
+    const bool may_list = temp > 0.f && by_count && k <= kSubPieces;
     float first[kCollectAhead], sub = 0.f;
     if (may_list) {
 #pragma unroll
@@ -483,7 +192,7 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
             const int j = threadIdx.x + 256 * i;
             first[i] = j < n ? row[begin + j] : -INFINITY;
         }
-        if (!by_least && threadIdx.x < kSubPieces) sub = sub_val[r * kSubPieces + threadIdx.x];
+        if (threadIdx.x < kSubPieces) sub = sub_val[r * kSubPieces + threadIdx.x];
     }
     const BestToken best = best_of_pieces(piece_val, piece_idx, r, threadIdx.x % kWave);
     if (c == 0 && threadIdx.x == 0) best_out[r] = best.index;
@@ -492,10 +201,9 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
     const float inv_t = 1.0f / fmaxf(temp, 1e-6f);
     if (may_list) {
         if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
-        const float bound_t = by_least ? logf(least) : exponent_of(bound_of_row(sub, k, s_sub, &s_bound), mx, inv_t);
-        if (by_least) __syncthreads();                       // (s_n is zeros, for everybody; the bound's search waits as well)
+        const float bound_t = exponent_of(bound_of_row(sub, k, s_sub, &s_bound), mx, inv_t);
         if (bound_t >= kLeastExponent && fabsf(mx) < INFINITY) {
-            collect_candidates(row, begin, n, first, mx, inv_t, bound_t, by_least ? least : 0.f, cand_w + static_cast<size_t>(r) * vocab,
+            collect_candidates(row, begin, n, first, mx, inv_t, bound_t, cand_w + static_cast<size_t>(r) * vocab,
                                cand_idx + static_cast<size_t>(r) * vocab, s_n);
             if (c == 0 && threadIdx.x == 0) listed[r] = 1;
             __syncthreads();
@@ -553,21 +261,20 @@ struct SamplePlan {
     int direct_piece;                   // without cuts: the piece that holds the drawn point, and what is left of it there
     unsigned long long direct_target;   // (top-p without top-k: the mass of the bins above `last`, from which its search goes on)
 };
-constexpr unsigned long long kAllPass = ~0ull;      // (in direct_target's place: nothing of the list is cut by top-p)
 struct SamplePlanSpace {
     unsigned int count[kSamplePieces][kTopBins + 1];
     unsigned long long mass[kSamplePieces][kTopBins + 1], bin_mass[kTopBins + 1];
     unsigned int bin_count[kTopBins + 1];
     int last, start[kSamplePieces + 1];
 };
-__device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, float least, float u, const unsigned int* __restrict__ piece_count,
+__device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, float u, const unsigned int* __restrict__ piece_count,
                                                   const unsigned long long* __restrict__ piece_mass, int vocab, SamplePlanSpace& space) {
     SamplePlan plan{kTopBins, 0, 0, 0, 0ull, -1, 0ull};
     const int t = threadIdx.x;
-    const bool by_count = k > 0 && k < vocab, by_mass = p > 0.f && p < 1.f, by_least = least > 0.f;
+    const bool by_count = k > 0 && k < vocab, by_mass = p > 0.f && p < 1.f;
     const unsigned int* counts = piece_count + static_cast<size_t>(r) * kSamplePieces * (kTopBins + 1);
     const unsigned long long* masses = piece_mass + static_cast<size_t>(r) * kSamplePieces * (kTopBins + 1);
-    if (!by_count && !by_mass && !by_least) {
+    if (!by_count && !by_mass) {
         // The pieces' masses are known, so the drawn point (in fixed point, of the whole row's mass) names its piece and what is
         // left of it inside that piece; the last kernel walks that piece alone.  (Every wavefront finds the same.)
         const int lane = t % kWave;
@@ -625,7 +332,6 @@ __device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, 
             for (int i = 0; i <= kTopBins; ++i) total += space.bin_mass[i];
             unsigned long long need = static_cast<unsigned long long>(static_cast<double>(p) * static_cast<double>(total));
             if (need == 0ull) need = 1ull;
-            if (!by_mass) need = ~0ull;                      // (min_p alone cuts)
             unsigned long long over = 0ull;
             for (int i = 0; i <= kTopBins; ++i) {
                 if (cum < need) {
@@ -636,11 +342,6 @@ __device__ __forceinline__ SamplePlan plan_of_row(int r, int c, int k, float p, 
             }
             space.bin_mass[0] = total;
             space.bin_mass[1] = over;
-            // below min_p's bin nothing is kept; the mass p is then not reached within the list, and all of it passes top-p
-            if (by_least && top_bin_of(__float_as_uint(least)) < last) {
-                last = top_bin_of(__float_as_uint(least));
-                space.bin_mass[1] = kAllPass;
-            }
         }
         space.last = last;
     }
@@ -680,7 +381,7 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
                                                              unsigned long long* __restrict__ row_mass,
                                                              int32_t* __restrict__ direct_piece,
                                                              unsigned long long* __restrict__ direct_target,
-                                                             int32_t* __restrict__ last_bin, int vocab, const float* __restrict__ min_p) {
+                                                             int32_t* __restrict__ last_bin, int vocab) {
     __shared__ int s_wave[4];
     __shared__ SamplePlanSpace s_plan;
     const int r = blockIdx.x, c = blockIdx.y;
@@ -693,13 +394,12 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
     const float* row = logits + static_cast<size_t>(r) * vocab;
     const float mx = row[best[r]];
     const float inv_t = 1.0f / fmaxf(temp, 1e-6f);
-    const float least = least_of(min_p, r);
     {
         const int k = top_k[r];
         const float p = top_p[r];
-        if (c > 0 && !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f) && !(least > 0.f)) return;      // no list is made without cuts
+        if (c > 0 && !(k > 0 && k < vocab) && !(p > 0.f && p < 1.f)) return;      // no list is made without cuts
     }
-    SamplePlan plan = plan_of_row(r, c, top_k[r], top_p[r], least, uniform[r], piece_count, piece_mass, vocab, s_plan);
+    SamplePlan plan = plan_of_row(r, c, top_k[r], top_p[r], uniform[r], piece_count, piece_mass, vocab, s_plan);
     if (!(fabsf(mx) < INFINITY)) {                           // an infinity or nothing but NaN: the row's best token and no draw
         plan.total = 0;
         plan.last = plan.direct_piece = -1;
@@ -775,7 +475,7 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
 // iff the mass of the greater weights is below it: the same sets as the thresholds of select_by_count and
 // select_by_mass (ties whole).  Counts and fixed-point masses are integers, so nothing depends on an order; the
 // draw walks the kept weights in index order.  Returns the picked position in the list or -1 (every thread).
-__device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool cut_by_count, unsigned int k, float p, float least,
+__device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool cut_by_count, unsigned int k, float p,
                                     bool mass_of_row, unsigned long long row_mass, float u, float* s_list /* [kSampleThreads] */,
                                     unsigned long long* s_wave /* [16] */, float* s_piece /* [16] */, int* s_pick /* [2] */) {
     __shared__ __attribute__((aligned(16))) unsigned long long s_fixed[kSampleThreads];
@@ -808,7 +508,6 @@ __device__ int pick_from_short_list(float wj /* of thread j < n */, int n, bool 
         if (need == 0ull) need = 1ull;
         keep = keep && mass_above < need;
     }
-    keep = keep && wj >= least;
     // inverse CDF in index order: prefix sums inside the wavefronts, then over them
     const float mine = keep ? wj : 0.f;
     float incl = mine;
@@ -913,8 +612,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     const float* __restrict__ top_p, const float* __restrict__ uniform, int32_t* __restrict__ out,
     float* __restrict__ weights, int vocab, const int32_t* __restrict__ cand_idx, const int32_t* __restrict__ cand_count,
     const int32_t* __restrict__ listed, const int32_t* __restrict__ list_count, const int32_t* __restrict__ best_in, const unsigned long long* __restrict__ row_mass,
-    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin,
-    const float* __restrict__ min_p) {
+    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin) {
     __shared__ float s_val[16];
     __shared__ int s_idx[16];
     __shared__ unsigned int hist[256];
@@ -934,7 +632,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     float* w = weights + static_cast<size_t>(r) * vocab;
     const int32_t* idx_of = cand_idx ? cand_idx + static_cast<size_t>(r) * vocab : nullptr;
     // (a row's few numbers at once: behind the branches that ask for them each would be a wait of its own)
-    const float temp = temperature[r], p = top_p[r], u = uniform[r], least = least_of(min_p, r);
+    const float temp = temperature[r], p = top_p[r], u = uniform[r];
     const int k = top_k[r];
     int known_best = 0, is_listed = 0, direct = -1, count = 0, more = 0;
     if (cand_idx) {
@@ -999,8 +697,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
             const float wj = j < n ? s_list[j] : 0.f;
             const int ij = j < n ? s_order[j] : 0x7fffffff;
             __syncthreads();
-            // (a list by min_p: all of it)
-            vocab = order_candidates(wj, ij, n, k > 0 && k < full_vocab ? static_cast<unsigned int>(k) : 0xffffffffu, s_list, s_order, hist);
+            vocab = order_candidates(wj, ij, n, static_cast<unsigned int>(k), s_list, s_order, hist);
         } else {
             // more than a thousand equals: the thresholds from the list, brought together in the first piece's place and behind it
             // (every piece's part moves towards the front, one piece after the other), the draw from the row
@@ -1028,15 +725,16 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     const unsigned long long mass = cand_idx && !k_active ? row_mass[r] : 0ull;
     if (vocab <= kSampleThreads) {                   // a short row or list: one thread per token
         const float wj = unordered ? s_list[threadIdx.x] : static_cast<int>(threadIdx.x) < vocab ? w[threadIdx.x] : 0.f;
-        const int at = pick_from_short_list(wj, vocab, k_active && k < vocab, static_cast<unsigned int>(k), p, least,
+        const int at = pick_from_short_list(wj, vocab, k_active && k < vocab, static_cast<unsigned int>(k), p,
                                             cand_idx && !k_active, mass, u, s_list, s_wave, s_piece, s_pick);
         if (threadIdx.x == 0) out[r] = at < 0 ? best : unordered ? s_order[at] : idx_of ? idx_of[at] : at;
         return;
     }
+    auto each_weight = [&](auto f) { for_each_in_row(w, vocab, threadIdx.x, blockDim.x, f); };
     // kept set = { j : w_j >= threshold }; the threshold starts at 0 (everything)
     uint32_t threshold = 0u;
     if (k_active && k < vocab)        // (a list of exactly k candidates is the top k)
-        threshold = select_by_count(w, vocab, static_cast<unsigned int>(k), hist, &s_a, &s_need);
+        threshold = select_by_count(each_weight, static_cast<unsigned int>(k), hist, &s_a, &s_need);
     if (p > 0.f && p < 1.f) {
         // mass of what top-k kept, in fixed point: per-thread sums, then over the wavefronts in order
         unsigned long long mine = 0ull;
@@ -1062,10 +760,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
             top = bin == 0 ? 0x3f800001u : static_cast<uint32_t>(128 - min(bin, kTopBins)) << 23;
             above = direct_target[r];
         }
-        if (above == kAllPass) threshold = 0u;
-        else threshold = select_by_mass(w, vocab, threshold, top, above, need, s_wave, &s_a, &s_b, &s_above);
+        threshold = select_by_mass(each_weight, threshold, top, above, need, s_wave, &s_a, &s_b, &s_above);
     }
-    threshold = max(threshold, __float_as_uint(least));
     // inverse CDF in index order.  Every wavefront owns a contiguous piece of the row; the piece that holds the
     // drawn point is then walked 64 tokens at a time with a prefix sum over the lanes.
     if (unordered) vocab = full_vocab;
@@ -1191,12 +887,12 @@ extern "C" int egpt_argmax_static(const float* logits, int32_t* out, int n_rows,
 
 // weights: scratch for n_rows * vocab floats.
 extern "C" int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                           const float* min_p, const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream) {
+                           const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !weights || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
     sample_kernel<<<n_rows, kSampleThreads, 0, static_cast<hipStream_t>(stream)>>>(
-        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, min_p);
+        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }
@@ -1217,7 +913,7 @@ extern "C" size_t egpt_sample_workspace(int n_rows, int vocab) {
 }
 
 extern "C" int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                                const float* min_p, const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream) {
+                                const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !workspace || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
@@ -1243,15 +939,14 @@ extern "C" int egpt_sample_wide(const float* logits, const float* temperature, c
     argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, sub, vocab);
     EGPT_CHECK_LAUNCH();
     sample_count_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, pv, pi, sub, best, listed, list_count, cand_w, cand_idx,
-                                                                    piece_count, piece_mass, vocab, top_p, min_p);
+                                                                    piece_count, piece_mass, vocab);
     EGPT_CHECK_LAUNCH();
     sample_compact_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, top_p, uniform, best, piece_count,
                                                                       piece_mass, listed, cand_w, cand_idx, cand_count, row_mass,
-                                                                      direct_piece, direct_target, last_bin, vocab, min_p);
+                                                                      direct_piece, direct_target, last_bin, vocab);
     EGPT_CHECK_LAUNCH();
     sample_kernel<<<n_rows, kSampleThreads, 0, s>>>(logits, temperature, top_k, top_p, uniform, out, cand_w, vocab, cand_idx,
-                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin,
-                                                    min_p);
+                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }

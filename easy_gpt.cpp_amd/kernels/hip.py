@@ -109,8 +109,9 @@ class HipKernels(KernelBackend):
             "egpt_attention_any_tiled": [vp, vp, vp, vp, vp, i, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_attention_any_decode": [vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i, i, i, i, i, f, i, i, i, vp],
             "egpt_argmax": [vp, vp, vp, i, i, vp],
-            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
-            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample_min_p": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
             "egpt_tree_attention_generic": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_tree_attention": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, i, i, i, i, vp],
             "egpt_accept_drafts": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp],
@@ -2178,18 +2179,29 @@ class HipKernels(KernelBackend):
 
     def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None):
         r, v = logits.shape
+        if min_p is not None:
+            self._here(logits, "logits", _F32)
+            device = logits.get_device()
+            self._lists(device, _F32, r, (temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform"), (min_p, "min_p"))
+            self._lists(device, _I32, r, (top_k, "top_k"), (out, "out"))
+            if r > 0:
+                self._run("egpt_sample_min_p", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+                          uniform.data_ptr(), out.data_ptr(), r, v, self._stream())
+            return
         self._need(logits, "logits", _F32)
-        device = logits.get_device()
-        self._lists(device, _F32, r, (temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform"), *(() if min_p is None else ((min_p, "min_p"),)))
-        self._lists(device, _I32, r, (top_k, "top_k"), (out, "out"))
+        self._need(temperature, "temperature", _F32, (r,))
+        self._need(top_k, "top_k", _I32, (r,))
+        self._need(top_p, "top_p", _F32, (r,))
+        self._need(uniform, "uniform", _F32, (r,))
+        self._need(out, "out", _I32, (r,))
         if v >= 8192:
             # a wide vocabulary: the row-wide passes by many workgroups, the selection on the tokens that are left
             space = torch.empty(int(self.lib.egpt_sample_workspace(r, v)), dtype=torch.uint8, device=logits.device)
-            self._run("egpt_sample_wide", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), self._ptr(min_p),
+            self._run("egpt_sample_wide", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
                       uniform.data_ptr(), out.data_ptr(), space.data_ptr(), r, v, self._stream())
             return
         weights = torch.empty((r, v), dtype=_F32, device=logits.device)
-        self._run("egpt_sample", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), self._ptr(min_p),
+        self._run("egpt_sample", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
                   uniform.data_ptr(), out.data_ptr(), weights.data_ptr(), r, v, self._stream())
 
     # ------------------------------------------------------------------ drafted tokens
