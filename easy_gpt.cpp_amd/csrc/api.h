@@ -400,9 +400,11 @@ size_t egpt_sample_workspace(int n_rows, int vocab);
 int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
                      const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream);
 // With a cut more (sampling_least.hip): min_p float32 [n_rows], of what top-k and top-p keep the tokens at least min_p times as likely as the
-// most likely one.  Any vocabulary below 2^23, no workspace.
+// most likely one.  A row is cut into `pieces` <= 1,024 of at most 32,768 tokens (three fewer where rows begin between 16 bytes); workspace:
+// egpt_sample_min_p_workspace(n_rows, pieces) bytes of device memory, null for one piece.  Vocabularies below 2^23.
+size_t egpt_sample_min_p_workspace(int n_rows, int pieces);
 int egpt_sample_min_p(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                      const float* uniform, int32_t* out, int n_rows, int vocab, void* stream);
+                      const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, int pieces, void* stream);
 
 // ---- drafted tokens (attention_tree.hip, drafts.hip)
 // Attention for trees: operands as egpt_paged_attention; the last q_len[b] of a request's kv_len[b] tokens are its nodes.  visible int64

@@ -111,7 +111,7 @@ class HipKernels(KernelBackend):
             "egpt_argmax": [vp, vp, vp, i, i, vp],
             "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
             "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
-            "egpt_sample_min_p": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
+            "egpt_sample_min_p": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp],
             "egpt_tree_attention_generic": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_tree_attention": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, i, i, i, i, vp],
             "egpt_accept_drafts": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp],
@@ -156,6 +156,8 @@ class HipKernels(KernelBackend):
         lib.egpt_decay_chunk.argtypes = [i, i]
         lib.egpt_sample_workspace.restype = ctypes.c_size_t
         lib.egpt_sample_workspace.argtypes = [i, i]
+        lib.egpt_sample_min_p_workspace.restype = ctypes.c_size_t
+        lib.egpt_sample_min_p_workspace.argtypes = [i, i]
         for name, argtypes in sigs.items():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
@@ -2177,6 +2179,22 @@ class HipKernels(KernelBackend):
         scratch = torch.empty(r * 64, dtype=_F32, device=logits.device) if v >= 8192 else None
         self._run("egpt_argmax", logits.data_ptr(), out.data_ptr(), self._ptr(scratch), r, v, self._stream())
 
+    @staticmethod
+    def _sample_pieces(rows: int, vocab: int, aligned: bool) -> int:
+        """How many pieces sampling with min-p makes of a row.  One workgroup takes a row that its registers hold, 32,768 tokens (three fewer where
+        rows begin between 16 bytes), by one launch; a longer row is of pieces of 8,192 as long as the device runs all of them at a time, two
+        workgroups a compute unit, beyond that of 32,768 (tokens of 151,936, us with 19 and with 5 pieces a row: 1 row 7.7 and 9.5, 16 rows 9.7 and
+        10.9, 32 rows 14.4 and 13.8, 256 rows 38 and 32; of 32,768 with 5 pieces and with 1: 1 row 9.4 and 8.2, 256 rows 19.3 and 11.7)."""
+        off = 0 if aligned else 3
+        if vocab <= 32768 - off:
+            return 1
+        small = -(-vocab // (8192 - off))
+        return small if rows * small <= 512 else -(-vocab // (32768 - off))
+
+    @functools.lru_cache(maxsize=4096)
+    def _sample_space(self, rows: int, pieces: int) -> int:
+        return int(self.lib.egpt_sample_min_p_workspace(rows, pieces))
+
     def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None):
         r, v = logits.shape
         if min_p is not None:
@@ -2185,8 +2203,10 @@ class HipKernels(KernelBackend):
             self._lists(device, _F32, r, (temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform"), (min_p, "min_p"))
             self._lists(device, _I32, r, (top_k, "top_k"), (out, "out"))
             if r > 0:
+                pieces = self._sample_pieces(r, v, v % 4 == 0 and logits.data_ptr() % 16 == 0)
+                space = torch.empty(self._sample_space(r, pieces), dtype=torch.uint8, device=logits.device) if pieces > 1 else None
                 self._run("egpt_sample_min_p", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
-                          uniform.data_ptr(), out.data_ptr(), r, v, self._stream())
+                          uniform.data_ptr(), out.data_ptr(), self._ptr(space), r, v, pieces, self._stream())
             return
         self._need(logits, "logits", _F32)
         self._need(temperature, "temperature", _F32, (r,))

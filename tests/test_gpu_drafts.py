@@ -382,6 +382,68 @@ def test_min_p_with_infinities_and_rows_of_nothing_but_nan(vocab):
         assert got[0] == 7 and got[1] == 0 and got[2] % 2 == 1 and not (5 <= got[3] < 50), (cuts, got)
 
 
+def test_rows_of_any_number_of_pieces_agree(monkeypatch):
+    # rows that begin between 16 bytes, pieces of a few tokens and of as many as they may have: the tokens are the same
+    g = torch.Generator().manual_seed(9)
+    n, vocab = 12, 70001
+    x = torch.randn((n, vocab), generator=g) * 2.5
+    x[3] *= 0.01
+    x[5, 100:60000] = -math.inf
+    x[6, 69000:] = math.nan
+    u = torch.rand((n,), generator=g)
+    k = kernels.backend()
+    for cuts in ((0, 1.0, 0.05), (50, 0.9, 0.05), (300, 1.0, 0.0), (0, 0.8, 0.01), (1000, 0.9, 1e-6)):
+        want = sample(x, 0.9, cuts[0], cuts[1], u, cuts[2])
+        for r in range(n):
+            if r not in (3, 5, 6) and far_from_borders(x[r], float(torch.tensor(0.9, dtype=F32)), cuts[0], float(torch.tensor(cuts[1], dtype=F32)), float(u[r]),
+                                                       float(torch.tensor(cuts[2], dtype=F32))):
+                assert want[r] == plain.sample_row(x[r].tolist(), float(torch.tensor(0.9, dtype=F32)), cuts[0], float(torch.tensor(cuts[1], dtype=F32)), float(u[r]),
+                                                   float(torch.tensor(cuts[2], dtype=F32))), (cuts, r)
+        for pieces in (3, 4, 9, 17, 40, 100, 1024):
+            with monkeypatch.context() as m:
+                m.setattr(k, "_sample_pieces", lambda *a: pieces, raising=False)
+                got = sample(x, 0.9, cuts[0], cuts[1], u, cuts[2])
+            assert got == want, (cuts, pieces)
+        one = x[:, :32765].contiguous()
+        want = sample(one, 0.9, cuts[0], cuts[1], u, cuts[2])
+        for pieces in (2, 13):
+            with monkeypatch.context() as m:
+                m.setattr(k, "_sample_pieces", lambda *a: pieces, raising=False)
+                got = sample(one, 0.9, cuts[0], cuts[1], u, cuts[2])
+            assert got == want, (cuts, pieces)
+
+
+@pytest.mark.parametrize("vocab", [650, 32768, 32766, 151936])
+def test_min_p_replayed_from_a_graph_and_on_another_stream(vocab):
+    n, k = 6, kernels.backend()
+    g = torch.Generator().manual_seed(11)
+    xs = [(torch.randn((n, vocab), generator=g) * 2.5).to(DEV) for _ in range(3)]
+    full = lambda v, dt=F32: torch.full((n,), v, dtype=dt, device=DEV)
+    x, temp, top_k, top_p, min_p, u = xs[0].clone(), full(0.8), full(30, torch.int32), full(0.9), full(0.03), torch.rand((n,), generator=g).to(DEV)
+
+    def eager(x):
+        out = torch.empty(n, dtype=torch.int32, device=DEV)
+        k.sample(x, temp, top_k, top_p, u, out, min_p=min_p)
+        return out.tolist()
+
+    want = [eager(v) for v in xs]
+    side, out = torch.cuda.Stream(), torch.empty(n, dtype=torch.int32, device=DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        k.sample(x, temp, top_k, top_p, u, out, min_p=min_p)
+    side.synchronize()
+    assert out.tolist() == want[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k.sample(x, temp, top_k, top_p, u, out, min_p=min_p)
+    for v, w in list(zip(xs, want)) * 2:
+        x.copy_(v)
+        out.fill_(-1)
+        graph.replay()
+        assert eager(xs[1]) == want[1]
+        assert out.tolist() == w
+
+
 def test_rows_of_one_call_have_cuts_of_their_own():
     g = torch.Generator().manual_seed(6)
     n, vocab = 40, 30000
