@@ -1,6 +1,7 @@
 // What follows the check of drafted tokens: the walk that takes those the model agrees with, and the move of their keys and values.
 #include "api.h"
 #include "common.h"
+#include "lds_loads.h"
 
 namespace egpt {
 
@@ -38,10 +39,18 @@ __global__ __launch_bounds__(64) void accept_drafts_kernel(const int32_t* __rest
 }
 
 // Entry path[b][k] of the tree goes to place k behind the start[b] tokens before it, key and value of every slab and kv head.  A path
-// ascends (a child lies behind its parent), so path[k] >= k: entries are moved in their order, a batch read before any of it is written, and no entry is
-// written over that a later one still has to be read from.  One workgroup per (request, slab); a thread owns the same 16 bytes of all keys, or
-// one feature of all values, so nobody waits for anybody.  (Values lie feature by feature: an entry is hd elements page_size apart, each a line of memory of its own.)
-constexpr int kMoveAhead = 8;
+// ascends (a child lies behind its parent), so path[k] >= k: entries are moved in their order, what is read together before any of it is written, and no
+// entry is written over that a later one still has to be read from.  One workgroup per (request, slab); a thread owns the same 16 bytes of all keys, or one
+// feature of all values, so nobody waits for anybody.
+//
+// Values lie feature by feature, an entry is hd elements page_size apart: written one by one they are a few bytes here and there of every line of a page, which
+// costs memory more than whole lines do.  Where 16 bytes of a feature's row lie in one page (pages of whole 16 bytes a row) a thread writes
+// those, the places between as they were.  64 users with 395 of 1,024 entries to move, 28 slabs of 2 heads of 128: 36.7 -> 21.2 us (by 32 bytes
+// 22.8); what is left is the pages' lines, 128 bytes for each 16 that change.  No two requests of a call may write into one page.
+constexpr int kMoveAhead = 16;          // entries read before the first is written: a trip to memory for most paths
+constexpr int kRowAhead = 3;            // 16 bytes of a feature's row likewise
+constexpr int kMostRows = kTreeNodes / 4 + 1;
+
 template <typename U>
 __device__ __forceinline__ void move_entries(U* __restrict__ base, const long long* s_from, const long long* s_to, int n, size_t at) {
     for (int k0 = 0; k0 < n; k0 += kMoveAhead) {
@@ -55,14 +64,49 @@ __device__ __forceinline__ void move_entries(U* __restrict__ base, const long lo
     }
 }
 
-// KU: the unit that keys are moved by; VU: a value.  k_units: units of a key (of one head).
-template <typename KU, typename VU>
+// The same for one feature of the values, 16 bytes of its row at a time: s_row where they lie, s_place the elements that come into each of their places (-1: it
+// stays as it is).
+template <typename U>
+__device__ __forceinline__ void move_rows(U* __restrict__ base, const long long* s_row, const long long (*s_place)[16 / sizeof(U)], int n, size_t at) {
+    constexpr int kIn = 16 / sizeof(U);
+    for (int k0 = 0; k0 < n; k0 += kRowAhead) {
+        U v[kRowAhead][kIn];
+        u32x4 was[kRowAhead];
+#pragma unroll
+        for (int k = 0; k < kRowAhead; ++k) {
+            if (k0 + k >= n) continue;
+            was[k] = *reinterpret_cast<const u32x4*>(base + s_row[k0 + k] + at);
+#pragma unroll
+            for (int e = 0; e < kIn; ++e) {
+                const long long from = s_place[k0 + k][e];
+                if (from >= 0) v[k][e] = base[from + at];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kRowAhead; ++k) {
+            if (k0 + k >= n) continue;
+            uint32_t w[4] = {was[k].x, was[k].y, was[k].z, was[k].w};
+#pragma unroll
+            for (int e = 0; e < kIn; ++e) {
+                if (s_place[k0 + k][e] < 0) continue;
+                if constexpr (sizeof(U) == 4) w[e] = v[k][e];
+                else w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | static_cast<uint32_t>(v[k][e]) << 16 : (w[e / 2] & 0xffff0000u) | v[k][e];
+            }
+            *reinterpret_cast<u32x4*>(base + s_row[k0 + k] + at) = u32x4{w[0], w[1], w[2], w[3]};
+        }
+    }
+}
+
+// KU: the unit that keys are moved by; VU: a value; kRows: values by 16 bytes of a row.  k_units: units of a key (of one head).
+template <typename KU, typename VU, bool kRows>
 __global__ __launch_bounds__(256) void keep_drafts_kernel(const int32_t* __restrict__ path, const int32_t* __restrict__ count,
                                                           const int32_t* __restrict__ start, const int32_t* __restrict__ block_table,
                                                           int path_width, int table_width, int n_pages, int page_size, int nkv, int k_units, int dv,
                                                           KU* __restrict__ k_cache, VU* __restrict__ v_cache) {
+    constexpr int kIn = 16 / sizeof(VU);
     __shared__ long long s_from_k[kTreeNodes], s_to_k[kTreeNodes], s_from_v[kTreeNodes], s_to_v[kTreeNodes];
-    __shared__ int s_n;
+    __shared__ long long s_row[kMostRows], s_place[kMostRows][kIn];
+    __shared__ int s_n, s_rows;
     const int b = blockIdx.x;
     if (threadIdx.x < kWave) {
         const int lane = threadIdx.x;
@@ -78,16 +122,29 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(const int32_t* __restr
             to = table[into / page_size];
         }
         moves = moves && from >= 0 && from < n_pages && to >= 0 && to < n_pages;
-        const unsigned long long all = __ballot(moves);
+        const unsigned long long all = __ballot(moves), up_to_me = (2ull << lane) - 1ull;
+        const long long kf = static_cast<long long>(from) * nkv * page_size, kt = static_cast<long long>(to) * nkv * page_size;
         if (moves) {
-            const int k = __popcll(all & ((1ull << lane) - 1ull));
-            const long long kf = static_cast<long long>(from) * nkv * page_size, kt = static_cast<long long>(to) * nkv * page_size;
+            const int k = __popcll(all & up_to_me) - 1;
             s_from_k[k] = (kf + of % page_size) * k_units;
             s_to_k[k] = (kt + into % page_size) * k_units;
             s_from_v[k] = kf * dv + of % page_size;
             s_to_v[k] = kt * dv + into % page_size;
         }
         if (lane == 0) s_n = __popcll(all);
+        if constexpr (kRows) {
+            for (int i = lane; i < kMostRows * kIn; i += kWave) (&s_place[0][0])[i] = -1;
+            // the first of the entries that go to the same 16 bytes of a row, places before + lane (16 bytes begin at multiples of kIn: pages do)
+            const int place = into % kIn, first = lane - place;                             // (the lane of their first place)
+            const unsigned long long earlier = all & ((1ull << lane) - 1ull) & (first > 0 ? ~0ull << first : ~0ull);
+            const unsigned long long heads = __ballot(moves && earlier == 0ull);
+            if (moves) {
+                const int row = __popcll(heads & up_to_me) - 1;
+                s_row[row] = kt * dv + into % page_size - place;
+                s_place[row][place] = kf * dv + of % page_size;
+            }
+            if (lane == 0) s_rows = __popcll(heads);
+        }
     }
     __syncthreads();
     const int n = s_n;
@@ -95,11 +152,14 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(const int32_t* __restr
     const size_t slab = static_cast<size_t>(blockIdx.y) * n_pages * nkv * page_size;
     const int keys = nkv * k_units, values = nkv * dv;
     for (int i = threadIdx.x; i < keys + values; i += 256) {
-        if (i < keys) {
-            const int h = i / k_units;
-            move_entries(k_cache + slab * k_units, s_from_k, s_to_k, n, static_cast<size_t>(h) * page_size * k_units + i % k_units);
+        if (i < values) {
+            VU* base = v_cache + slab * dv;
+            const size_t at = static_cast<size_t>(i) * page_size;
+            if constexpr (kRows) move_rows(base, s_row, s_place, s_rows, at);
+            else move_entries(base, s_from_v, s_to_v, n, at);
         } else {
-            move_entries(v_cache + slab * dv, s_from_v, s_to_v, n, static_cast<size_t>(i - keys) * page_size);
+            const int h = (i - values) / k_units;
+            move_entries(k_cache + slab * k_units, s_from_k, s_to_k, n, static_cast<size_t>(h) * page_size * k_units + (i - values) % k_units);
         }
     }
 }
@@ -129,19 +189,21 @@ extern "C" int egpt_keep_drafts(void* k_cache, void* v_cache, const int32_t* blo
     if (n_seqs == 0 || n_slabs == 0 || n_pages == 0) return EGPT_OK;
     const dim3 grid(n_seqs, n_slabs);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const int size = dtype == 0 ? 4 : 2, key_bytes = dk * size;
+    const bool rows = page_size * size % 16 == 0 && reinterpret_cast<uintptr_t>(v_cache) % 16 == 0;
     auto launch = [&](auto key, auto value, int k_units) {
         using KU = decltype(key);
         using VU = decltype(value);
-        keep_drafts_kernel<KU, VU><<<grid, 256, 0, s>>>(path, count, start, block_table, path_width, table_width, n_pages, page_size, nkv, k_units, dv,
-                                                       static_cast<KU*>(k_cache), static_cast<VU*>(v_cache));
+        auto kernel = rows ? keep_drafts_kernel<KU, VU, true> : keep_drafts_kernel<KU, VU, false>;
+        kernel<<<grid, 256, 0, s>>>(path, count, start, block_table, path_width, table_width, n_pages, page_size, nkv, k_units, dv,
+                                    static_cast<KU*>(k_cache), static_cast<VU*>(v_cache));
     };
-    const int key_bytes = dk * (dtype == 0 ? 4 : 2);
     const bool wide = key_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0;       // keys by 16 bytes
     if (dtype == 0) {
-        if (wide) launch(uint4{}, uint32_t{}, key_bytes / 16);
+        if (wide) launch(u32x4{}, uint32_t{}, key_bytes / 16);
         else launch(uint32_t{}, uint32_t{}, dk);
     } else {
-        if (wide) launch(uint4{}, uint16_t{}, key_bytes / 16);
+        if (wide) launch(u32x4{}, uint16_t{}, key_bytes / 16);
         else launch(uint16_t{}, uint16_t{}, dk);
     }
     EGPT_CHECK_LAUNCH();

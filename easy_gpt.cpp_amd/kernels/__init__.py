@@ -54,7 +54,7 @@ Methods of a backend (T tokens, B requests, R rows, act = bfloat16 or float32):
   keep_drafts(k_cache [slabs,P,nkv,page_size,dk] | [P,...], v_cache [slabs,P,nkv,dv,page_size] | [P,...], block_table i32[B,W],
               start i32[B], path i32[B,L], count i32[B])
         key and value of the first count[b] nodes of an ascending path, which lie at places start[b] + path[b,k] of their request, go to places
-        start[b] + k, in all slabs (in place; the other nodes' places hold what they held)
+        start[b] + k, in all slabs (in place; the other nodes' places hold what they held).  No page may take entries of two requests
 
   (head_norm_store, latent_prep and sigmoid_gate also take row_ss f32[S2,T], hidden, norm_eps: the product, float32
    partial sums, then still lacks each row's factor 1/sqrt(sum_s row_ss[s] / hidden + norm_eps), as `product_normed`
