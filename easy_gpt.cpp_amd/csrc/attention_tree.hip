@@ -6,6 +6,7 @@
 //     j = kv - n + m   and bit m of visible_i is set                 (node m; a request has at most 64)
 // and is softmax_j(scale q . k_j) v_j over those, zeros where there are none.  A number that a row does not see does not reach it, be it an
 // infinity or a NaN.
+#include <atomic>
 #include <type_traits>
 
 #include "api.h"
@@ -182,8 +183,8 @@ struct TreeSizes {
 
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 constexpr int tree_lds() {
-    constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = (KS - 1) * RB * 64 * (HD / 2 + 2) * 4;
-    return stages > join ? stages : join;
+    constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = KS * RB * 64 * (HD / 2 + 2) * 4;
+    return KS == 1 || stages > join ? stages : join;
 }
 
 // Which request's work a workgroup has: the requests' works lie one after the other, request b has work_of(q_len[b], kv_len[b]) of them.  Workgroups go to the eight
@@ -568,52 +569,74 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     }
     float l = fold_32_apart(l_run, AddOf());
 
-    if constexpr (KS > 1) {                      // the groups' results, joined in their order
-        float* const space = reinterpret_cast<float*>(smem);
-        __syncthreads();
-        if (ksi > 0) {
-            float* mine = space + static_cast<size_t>((ksi - 1) * RB + rb) * 64 * (HD / 2 + 2) + lane;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mine[(d * 16 + e) * 64] = acc[d][e];
-            mine[HD / 2 * 64] = m_run;
-            mine[(HD / 2 + 1) * 64] = l;
-        }
-        __syncthreads();
-        if (ksi > 0) return;
-#pragma unroll
-        for (int k = 1; k < KS; ++k) {
-            const float* from_k = space + static_cast<size_t>((k - 1) * RB + rb) * 64 * (HD / 2 + 2) + lane;
-            const float m_k = from_k[HD / 2 * 64], l_k = from_k[(HD / 2 + 1) * 64];
-            const float m_new = fmaxf(m_run, m_k);
-            const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale2);
-            const float c = m_k == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_k - m_new) * scale2);
-            l = l * a + l_k * c;
-            m_run = m_new;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * a + from_k[(d * 16 + e) * 64] * c;
-        }
-    }
-    if (!valid) return;
-    const size_t row = static_cast<size_t>(token) * z.nq + head;
+    // Four neighbouring features of a row are a quad: quad 4 d + e / 4 of a lane the ones from d * 32 + 2 e + 4 lh on.  The groups' results are joined, each group
+    // its share of the quads (one wavefront that joins them all is as long alone as two tiles: an instruction of a wavefront that has its SIMD to itself is 5 cycles).
+    const size_t row = static_cast<size_t>(token) * z.nq + head, mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
     const bool whole = n_parts == 1;
-    const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
-    const size_t mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
+    constexpr int QUADS = DB * 4, SHARE = QUADS / KS;
+    static_assert(QUADS % KS == 0, "as many quads for every group");
+    auto leave = [&](const float (&v)[4], int quad, float factor) {
+        const int at = quad / 4 * 32 + quad % 4 * 8 + lh * 4;
+        const float o[4] = {v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor};
+        if (at >= z.hd) return;
+        if (whole) write_quad(out + row * z.hd + at, o);
+        else write_quad(part_o + mine * z.hd + at, o);
+    };
+    float m_all = m_run;
+    if constexpr (KS > 1) {
+        tree_f32x4* const results = reinterpret_cast<tree_f32x4*>(smem) + static_cast<size_t>(rb) * QUADS * kWave + lane;         // [group][rb][quad][lane]
+        float2* const sums = reinterpret_cast<float2*>(smem + KS * RB * QUADS * kWave * 16) + rb * kWave + lane;                  // [group][rb][lane]
+        __syncthreads();
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = d * 32 + e * 2 + lh * 4;
-            const float v[4] = {acc[d][e] * inv, acc[d][e + 1] * inv, acc[d][e + 2] * inv, acc[d][e + 3] * inv};
-            if (at >= z.hd) continue;
-            if (whole) write_quad(out + row * z.hd + at, v);
-            else write_quad(part_o + mine * z.hd + at, v);
+            for (int e = 0; e < 4; ++e)
+                results[(ksi * RB * QUADS + d * 4 + e) * kWave] = tree_f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+        sums[ksi * RB * kWave] = float2{m_run, l};
+        __syncthreads();
+        float factor[KS], l_of[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const float2 one = sums[k * RB * kWave];
+            factor[k] = one.x;
+            l_of[k] = one.y;
         }
-    if (!whole && lh == 0) {
-        part_ml[mine * 2] = m_run * scale2;
+        m_all = factor[0];
+#pragma unroll
+        for (int k = 1; k < KS; ++k) m_all = fmaxf(m_all, factor[k]);
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            factor[k] = factor[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((factor[k] - m_all) * scale2);
+            l = fmaf(l_of[k], factor[k], l);
+        }
+        const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+        if (!valid) return;
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            const int quad = ksi * SHARE + i;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const tree_f32x4 one = results[(k * RB * QUADS + quad) * kWave];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(one[e], factor[k], v[e]);
+            }
+            leave(v, quad, inv);
+        }
+    } else {
+        if (!valid) return;
+        const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v[4] = {acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+                leave(v, d * 4 + e, inv);
+            }
+    }
+    if (!whole && lh == 0 && ksi == 0) {
+        part_ml[mine * 2] = m_all * scale2;
         part_ml[mine * 2 + 1] = l;
     }
 }
@@ -686,9 +709,15 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
     const long long grid = (works + 7) / 8 * 8;
     if (grid >= 1 << 27) return EGPT_UNSUPPORTED_SIZE;
     auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
-    if (lds > 60 * 1024) {
-        static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-        if (!raised) return EGPT_UNSUPPORTED_SIZE;
+    if (lds > 60 * 1024) {                                   // more than a launch may have unasked: asked for once per instance and device
+        static std::atomic<unsigned long long> raised{0};
+        int device = -1;
+        if (hipGetDevice(&device) != hipSuccess) return EGPT_LAUNCH_FAILED;
+        const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+        if ((raised.load(std::memory_order_relaxed) & bit) == 0ull) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return EGPT_LAUNCH_FAILED;
+            raised.fetch_or(bit, std::memory_order_relaxed);
+        }
     }
     kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, chunk, magic_of(chunk), group, max_q_len,
                                                                    table_width, q_start, static_cast<const T*>(qkv), visible, positions,
@@ -758,6 +787,7 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
         if (shape == 22) EGPT_TREE(bf16_t, 64, 2, 2, 64, 2);
         if (shape == 41) EGPT_TREE(bf16_t, 64, 4, 1, 64, 2);
     } else if (dtype == 1 && hd <= 128) {
+        if (shape == 14) EGPT_TREE(bf16_t, 128, 1, 4, 32, 2);
         if (shape == 22) EGPT_TREE(bf16_t, 128, 2, 2, 32, 2);
         if (shape == 81) EGPT_TREE(bf16_t, 128, 8, 1, 64, 3);
     } else if (dtype == 1) {

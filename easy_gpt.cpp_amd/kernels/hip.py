@@ -2298,11 +2298,11 @@ class HipKernels(KernelBackend):
     # many as it holds.  (By the fit's choice 3 % slower than the best of what was measured; 64 requests of 1 to 32 nodes behind 128 to 4,000 tokens 17 %,
     # whose sums it cannot know.)
     _tree_shapes = {
-        (1, 64): ((14, 128, 2, 5.95, 0.77, 1.28), (22, 128, 2, 5.46, 1.05, 1.68), (41, 64, 3, 5.2, 0.93, 1.15)),
-        (1, 128): ((22, 64, 2, 6.74, 1.03, 1.43), (81, 64, 1, 6.24, 1.96, 1.96)),
+        (1, 64): ((14, 128, 2, 5.4, 0.77, 1.27), (22, 128, 2, 5.44, 1.04, 1.66), (41, 64, 3, 5.21, 0.93, 1.13)),
+        (1, 128): ((14, 128, 1, 5.84, 1.44, 1.44), (22, 64, 2, 6.43, 1.04, 1.42), (81, 64, 1, 6.09, 1.91, 1.91)),
         (1, 256): ((12, 64, 1, 6.95, 2.25, 2.25), (41, 32, 1, 5.7, 2.08, 2.08)),
-        (0, 64): ((14, 128, 1, 5.12, 3.37, 3.37), (22, 64, 2, 6.39, 2.4, 4.75)),
-        (0, 128): ((22, 64, 1, 7.4, 4.86, 4.86), (41, 32, 2, 6.85, 4.14, 11.0)),
+        (0, 64): ((14, 128, 1, 4.7, 3.35, 3.35), (22, 64, 2, 6.51, 2.41, 4.75)),
+        (0, 128): ((22, 64, 1, 7.23, 4.85, 4.85), (41, 32, 2, 7.08, 4.06, 9.84)),
         (0, 256): ((41, 32, 1, 7.0, 8.0, 8.0),),
     }
 
@@ -2310,7 +2310,7 @@ class HipKernels(KernelBackend):
     @functools.lru_cache(maxsize=4096)
     def _tree_shape(cls, b, t, nkv, group, hd, dt, max_q_len, max_kv_len) -> tuple[int, int, int]:
         """(shape, parts of a request's keys at most, keys of a part) of the matrix-core kernel for trees: the cheapest by the fit.  The joining
-        kernel costs 2.9 us and 0.25 for a megabyte of the parts' results."""
+        kernel costs 3 us and 0.26 for a megabyte of the parts' results."""
         best = None
         for shape, keys, held, launch, alone, full in cls._tree_shapes[dt, 64 if hd <= 64 else 128 if hd <= 128 else 256]:
             rows = 32 * (shape // 10)
@@ -2326,7 +2326,7 @@ class HipKernels(KernelBackend):
                 turns = max(1, -(-works // (256 * held)))
                 us = launch + turns * per * (alone + (full - alone) * min(1.0, max(0.0, works / turns / 256 - 1) / max(held - 1, 1))) + (turns - 1) * 1.5
                 if parts > 1:
-                    us += 2.9 + 0.25e-6 * parts * t * group * nkv * hd * 8
+                    us += 3.0 + 0.26e-6 * parts * t * group * nkv * hd * 8
                 if best is None or us < best[0]:
                     best = us, shape, parts, per * keys
         return best[1:]
