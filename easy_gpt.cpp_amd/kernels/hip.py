@@ -2235,7 +2235,7 @@ class HipKernels(KernelBackend):
     def _lists(self, device: int, dtype, n: int, *named) -> None:
         """Tensors of n numbers each on that device."""
         for t, name in named:
-            if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
+            if not (isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype is dtype and t.shape == (n,) and t.is_contiguous()):
                 self._here(t, name, dtype, (n,))
 
     def _table(self, device: int, t, name: str) -> tuple[int, int]:
@@ -2256,16 +2256,27 @@ class HipKernels(KernelBackend):
             raise ValueError(f"a request's tree has at most {self.max_tree_nodes} nodes, not {max_q_len}")
         if window < 0:
             raise ValueError("the window must be >= 0")
-        self._here(qkv, "qkv")
-        if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * hd:
-            raise ValueError(f"qkv must be [tokens, {(nq + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
-        dt, dtype, device, t = self._act(qkv, "qkv"), qkv.dtype, qkv.get_device(), qkv.shape[0]
-        self._here(out, "out", dtype, (t, nq * hd))
-        self._here(k_cache, "k_cache", dtype)
-        self._here(v_cache, "v_cache", dtype)
-        pages = k_cache.shape[0]
-        if k_cache.shape != (pages, nkv, page_size, hd) or v_cache.shape != (pages, nkv, hd, page_size):
+        try:
+            t, dtype, device, pages = qkv.shape[0], qkv.dtype, qkv.get_device(), k_cache.shape[0]
+            usual = (dtype in _DT and device == torch._C._cuda_getDevice() and qkv.shape == (t, (nq + 2 * nkv) * hd) and qkv.is_contiguous()
+                     and out.get_device() == device and out.dtype is dtype and out.shape == (t, nq * hd) and out.is_contiguous()
+                     and k_cache.get_device() == device and k_cache.dtype is dtype and k_cache.shape == (pages, nkv, page_size, hd)
+                     and k_cache.is_contiguous() and v_cache.get_device() == device and v_cache.dtype is dtype
+                     and v_cache.shape == (pages, nkv, hd, page_size) and v_cache.is_contiguous())
+        except (AttributeError, IndexError):                 # (something that is no tensor, or has no sizes)
+            usual = False
+        if not usual:
+            self._here(qkv, "qkv")
+            if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * hd:
+                raise ValueError(f"qkv must be [tokens, {(nq + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
+            self._act(qkv, "qkv")
+            t, dtype, device = qkv.shape[0], qkv.dtype, qkv.get_device()
+            self._here(out, "out", dtype, (t, nq * hd))
+            self._here(k_cache, "k_cache", dtype)
+            self._here(v_cache, "v_cache", dtype)
             self._caches(k_cache, v_cache, dtype, nkv, page_size, hd)
+            pages = k_cache.shape[0]
+        dt = _DT[dtype]
         b, width = self._table(device, block_table, "block_table")
         self._lists(device, _I32, b, (q_start, "q_start"), (q_len, "q_len"), (kv_len, "kv_len"))
         self._lists(device, _I64, t, (visible, "visible"))
@@ -2281,7 +2292,7 @@ class HipKernels(KernelBackend):
         more = (block_table.data_ptr(), width, pages, q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
                 positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window))
         if hd * (4 if dt == 0 else 2) % 16 == 0 and page_size % 16 == 0 and not (at_q | at_out | at_k | at_v) & 15:
-            shape, parts, chunk = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 256) * 256)
+            shape, parts, chunk = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 64) * 64)
             part_o = part_ml = None
             if parts > 1:
                 rows = parts * t * nq

@@ -257,6 +257,14 @@ def test_attention_refusals():
     refused(TypeError, 0, c["qkv"].half())
     refused(ValueError, 0, c["qkv"][:, :-1])
     refused(TypeError, 0, c["qkv"].cpu())
+    refused(TypeError, 0, None)
+    refused(ValueError, 0, c["qkv"][0])
+    refused(TypeError, 1, None)
+    refused(TypeError, 2, None)
+    refused(ValueError, 2, c["k_cache"][:-1])
+    refused(TypeError, 3, [])
+    refused(TypeError, 4, None)
+    refused(TypeError, 8, None)
     refused(TypeError, 1, good[1].float())
     refused(ValueError, 1, good[1][:3])
     refused(TypeError, 2, c["k_cache"].float())
