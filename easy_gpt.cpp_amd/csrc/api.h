@@ -415,14 +415,15 @@ int egpt_tree_attention_generic(const void* qkv, void* out, const void* k_cache,
                                 const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,
                                 int dtype, void* stream);
 // The same on the matrix cores: keys of whole 16 bytes, page sizes that are multiples of 16, operands on 16 bytes.  No request brings more than max_q_len
-// <= 64 nodes.  A request's keys are cut into parts of `chunk`, a multiple of the shape's keys a round, at most `parts` <= 64 of them; with more than one,
-// part_o [parts][n_tokens][nq][hd] and part_ml [parts][n_tokens][nq][2] (float32) hold their results until a second kernel joins them.  shape: 10 * blocks
+// <= 64 nodes.  A request's keys are cut into at most `parts` <= 64 parts, so many that there are about `want`
+// workgroups; with parts > 1, part_o [parts][n_tokens][nq][hd] and part_ml [parts][n_tokens][nq][2] (float32) and one int behind the latter hold
+// their results until a second kernel joins them.  shape: 10 * blocks
 // of 32 rows that a workgroup takes + wavefronts that share a block's keys: bfloat16 up to head size 64 14, 22, 41, up to 128 14, 22, 81, beyond 12, 41;
 // float32 14, 22; 22, 41; 41.
 int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
                         int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
                         const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,
-                        int max_q_len, int shape, int parts, int chunk, int dtype, void* stream);
+                        int max_q_len, int shape, int parts, int want, int dtype, void* stream);
 // path, accepted int32 [n_seqs][64], count int32 [n_seqs]
 int egpt_accept_drafts(const int32_t* tokens, const int32_t* parents, const int32_t* sampled, const int32_t* q_start, const int32_t* q_len, int n_seqs,
                        int n_tokens, int32_t* path, int32_t* count, int32_t* accepted, void* stream);

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
 // resource with that page's base, bounded by it, and a constant offset per lane.  Keys lie in rows, 16-byte pieces exchanged by the row's number, values as a page of 16
 // tokens has them: either way 64 lanes read different banks.  A head that is no power of two is filled up with zeros by the loads' bounds.
 //
-// A request's keys are cut into parts of `chunk`, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
+// A request's keys are cut into parts, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
 // parts leave the unnormalised result with its maximum and sum, and tree_combine_kernel joins them.
 typedef __attribute__((ext_vector_type(8))) __bf16 tree_bf16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -187,15 +187,30 @@ constexpr int tree_lds() {
     return KS == 1 || stages > join ? stages : join;
 }
 
-// Which request's work a workgroup has: the requests' works lie one after the other, request b has work_of(q_len[b], kv_len[b]) of them.  Workgroups go to the eight
+// The rounds of `keys` (a power of two) keys that a context takes, one at least; contexts are below 2^27.
+__device__ __forceinline__ int rounds_of_keys(int kv, int keys) { return min(max(kv, 1) - 1, (1 << 27) - 1) / keys + 1; }
+// ceil(x / d), x and d below 2^22; inv a reciprocal of d.
+__device__ __forceinline__ int upper_quotient(int x, int d, float inv) {
+    const int y = x + d - 1, q = static_cast<int>(static_cast<float>(y) * inv);
+    return q + ((q + 1) * d <= y ? 1 : 0) - (q * d > y ? 1 : 0);
+}
+
+// Which request's work a workgroup has: a block of rows over a part of its keys, of `per` rounds (KT * KS keys each).  The host says how many works would be best if
+// every context were as long as the longest can be (`want`); here `per` follows from what the contexts are, so that there are about as many, and no request has more
+// than `most` parts.  (64 requests of 1 to 32 nodes behind 128 to 4,000 tokens: 43.1 us with parts of a length chosen
+// by the longest alone, 36.6 so.)
+//
+// The requests' works lie one after the other, request b has blocks_of(q_len[b]) * ceil(rounds_of(kv_len[b]) / per) of them.  Workgroups go to the eight
 // dies in turn, so those of a die take works that follow each other: blocks of rows that read the same keys are on one die.  As many workgroups as works, not
-// as the most of any request for each: workgroups without work, in a pattern, leave the same compute units idle (64 requests of 1 to 32 nodes
-// behind 128 to 4,000 tokens: 154 of 256 busy).  64 requests at a time, by a sum over the lanes.  False: nobody's.
+// as the most of any request for each: workgroups without work, in a pattern, leave the same compute units idle (154 of 256 busy there).
+// 64 requests at a time, by a sum over the lanes.  False: nobody's.
 struct TreeWork {
-    int request, index, n, kv;
+    int request, index, n, kv, per, parts;
+    bool first;
 };
-template <class F>
-__device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, int n_seqs, F work_of, TreeWork& found) {
+template <class Blocks, class Rounds>
+__device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, int n_seqs, Blocks blocks_of, Rounds rounds_of,
+                                          int want, int most, unsigned magic_most, TreeWork& found) {
     const int lane = threadIdx.x % kWave;
     auto upto_of = [&](int v) {
         v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);                // row_shr:1, 2, 4, 8: the sum within a row
@@ -206,15 +221,51 @@ __device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, con
         v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
         return v;
     };
-    int n = lane < n_seqs ? q_len[lane] : 0, kv = lane < n_seqs ? kv_len[lane] : 0;
-    int work = work_of(n, kv), upto = upto_of(work), total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    auto sum_of = [&](int v) { return __builtin_amdgcn_readlane(upto_of(v), kWave - 1); };
+    const int n0 = lane < n_seqs ? q_len[lane] : 0, kv0 = lane < n_seqs ? kv_len[lane] : 0;
+    const int blocks0 = blocks_of(n0), rounds0 = rounds_of(kv0);
+    int per = 1 << 21;                           // (one part of each: as many rounds as it takes)
+    if (most > 1 && n_seqs == 1) {               // (the host knew it all)
+        per = divided(__builtin_amdgcn_readfirstlane(rounds0) + most - 1, most, magic_most);
+    } else if (most > 1) {
+        int blocks = sum_of(blocks0);
+        float all = wave_sum(static_cast<float>(blocks0) * static_cast<float>(rounds0)), longest = blocks0 > 0 ? static_cast<float>(rounds0) : 0.f;
+        for (int s0 = kWave; s0 < n_seqs; s0 += kWave) {
+            const int i = s0 + lane, b = i < n_seqs ? blocks_of(q_len[i]) : 0, r = i < n_seqs ? rounds_of(kv_len[i]) : 0;
+            all += wave_sum(static_cast<float>(b) * static_cast<float>(r));
+            blocks += sum_of(b);
+            longest = fmaxf(longest, b > 0 ? static_cast<float>(r) : 0.f);
+        }
+        const int least = divided(__builtin_amdgcn_readfirstlane(static_cast<int>(wave_max(longest))) + most - 1, most, magic_most);
+        auto rounds_for = [&](int works) {                   // ceil(all / works)
+            const float w = static_cast<float>(works);
+            const int q = static_cast<int>(fminf(all * __builtin_amdgcn_rcpf(w), 2097152.f));
+            return q + (static_cast<float>(q) * w < all ? 1 : 0);
+        };
+        per = max(max(least, rounds_for(want)), 1);
+        // (parts that do not come out even are some half a part more for each block of rows)
+        const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+        int works = sum_of(blocks0 * upper_quotient(rounds0, per, inv));
+        for (int s0 = kWave; s0 < n_seqs; s0 += kWave) {
+            const int i = s0 + lane;
+            works += sum_of(i < n_seqs ? blocks_of(q_len[i]) * upper_quotient(rounds_of(kv_len[i]), per, inv) : 0);
+        }
+        if (works > want) per = max(per, rounds_for(max(want - blocks / 2, 1)));
+        per = __builtin_amdgcn_readfirstlane(per);
+    }
+    const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+    int n = n0, kv = kv0, parts = most > 1 ? upper_quotient(rounds0, per, inv) : 1, work = blocks0 * parts, upto = upto_of(work);
+    int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    auto parts_of = [&](int kv_) { return most > 1 ? upper_quotient(rounds_of(kv_), per, inv) : 1; };
     for (int s0 = kWave; s0 < n_seqs; s0 += kWave) {
         const int i = s0 + lane;
-        total += __builtin_amdgcn_readlane(upto_of(i < n_seqs ? work_of(q_len[i], kv_len[i]) : 0), kWave - 1);
+        total += sum_of(i < n_seqs ? blocks_of(q_len[i]) * parts_of(kv_len[i]) : 0);
     }
     const int each = (total + 7) / 8;
     int index = static_cast<int>(blockIdx.x % 8) * each + static_cast<int>(blockIdx.x / 8);
     if (static_cast<int>(blockIdx.x / 8) >= each || index >= total) return false;
+    found.per = per;
+    found.first = index == 0;
     for (int s0 = 0;;) {
         const unsigned long long behind = __ballot(upto > index);
         if (behind != 0) {
@@ -223,6 +274,7 @@ __device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, con
             found.index = index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(work, at));
             found.n = __builtin_amdgcn_readlane(n, at);
             found.kv = __builtin_amdgcn_readlane(kv, at);
+            found.parts = __builtin_amdgcn_readlane(parts, at);
             return true;
         }
         index -= __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -230,7 +282,8 @@ __device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, con
         const int i = s0 + lane;
         n = i < n_seqs ? q_len[i] : 0;
         kv = i < n_seqs ? kv_len[i] : 0;
-        work = work_of(n, kv);
+        parts = parts_of(kv);
+        work = blocks_of(n) * parts;
         upto = upto_of(work);
     }
 }
@@ -238,10 +291,10 @@ __device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, con
 // (the first 14 words of the arguments arrive with the wavefronts: all that the first trip to memory needs)
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1) void tree_attention_kernel(
-    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int n_seqs, int nkv, int parts,
-    int chunk, unsigned magic_chunk, int group, int max_q_len, int table_width, const int32_t* __restrict__ q_start,
+    const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int n_seqs, int nkv, int most_parts,
+    int want, int group, int max_q_len, int table_width, unsigned magic_most, const int32_t* __restrict__ q_start,
     const T* __restrict__ qkv, const long long* __restrict__ visible, const int32_t* __restrict__ positions, const T* __restrict__ k_cache,
-    const T* __restrict__ v_cache, T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml, TreeSizes z) {
+    const T* __restrict__ v_cache, T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ per_out, TreeSizes z) {
     constexpr int SZ = sizeof(T);
     constexpr int ROWB = HD * SZ, PIECES = ROWB / 16, KC = ROWB / 32, DB = HD / 32, KB = KT / 32;
     constexpr int HALF = KT * ROWB, TILE = 2 * HALF;             // bytes of a tile's keys, and of it all
@@ -257,12 +310,14 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 
     // which part of which request and kv head, and which block of its rows
     auto blocks_of = [&](int n_) { return (min(max(n_, 0), max_q_len) * group + 32 * RB - 1) / (32 * RB); };
-    auto parts_of = [&](int kv_) { return min(divided(max(kv_, 1) - 1, chunk, magic_chunk) + 1, parts); };
     TreeWork work;
-    if (!find_work(q_len, kv_len, n_seqs, [&](int n_, int kv_) { return blocks_of(n_) * parts_of(kv_) * nkv; }, work)) return;
-    const int b = work.request, n = work.n, kv_all = work.kv;
-    const int blocks = blocks_of(n), n_parts = parts_of(kv_all);
+    if (!find_work(q_len, kv_len, n_seqs, [&](int n_) { return blocks_of(n_) * nkv; }, [](int kv_) { return rounds_of_keys(kv_, KT * KS); }, want, most_parts,
+                   magic_most, work))
+        return;
+    const int b = work.request, n = work.n, kv_all = work.kv, chunk = work.per * (KT * KS);
+    const int blocks = blocks_of(n), n_parts = work.parts;
     const int unit = work.index / blocks, block = work.index - unit * blocks, kvh = unit / n_parts, part = unit - kvh * n_parts;
+    if (most_parts > 1 && work.first && tid == 0) *per_out = work.per;
     const int qs = q_start[b];
     const int from = part * chunk;
     // The pages of 64 groups of keys, a lane each, asked for before it is known how many keys there are; the next 64 while these are walked.
@@ -278,7 +333,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     Places here = places_from(from);
     const int rows = n * group, row0 = block * 32 * RB;
     const int before = kv_all - n, kv = min(kv_all, table_width * z.page_size);
-    const int to = min(kv, from + chunk);
+    const int to = min(kv - from, chunk) + from;
     const int groups = to > from ? (to - from + kGroup - 1) / kGroup : 0;
 
     const int key_bytes = z.hd * SZ;
@@ -646,13 +701,13 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 // that saw nothing weighs nothing, whatever it holds.
 template <typename T>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start,
-                                                           const float* __restrict__ part_ml, const float* __restrict__ part_o, int chunk, unsigned magic_chunk,
-                                                           int nq, unsigned magic_heads, int nodes, int most_parts, int n_tokens, int hd, T* __restrict__ out) {
+                                                           const float* __restrict__ part_ml, const float* __restrict__ part_o, const int* __restrict__ per_of, int round_keys,
+                                                           int nq, unsigned magic_heads, int nodes, int n_tokens, int hd, T* __restrict__ out) {
     constexpr int kAhead = 8;
     const int lane = threadIdx.x % kWave, w = blockIdx.x * 4 + threadIdx.x / kWave, b = blockIdx.y;
     const int node = divided(w, nq, magic_heads), head = w - node * nq;
     const int n = q_len[b], kv = kv_len[b], token = q_start[b] + node;
-    const int parts = min(divided(max(kv, 1) - 1, chunk, magic_chunk) + 1, most_parts);
+    const int per = *per_of, parts = upper_quotient(rounds_of_keys(kv, round_keys), per, __builtin_amdgcn_rcpf(static_cast<float>(per)));
     if (node >= n || node >= nodes || parts < 2 || token < 0 || token >= n_tokens) return;
     const size_t row = static_cast<size_t>(token) * nq + head, step = static_cast<size_t>(n_tokens) * nq;
     const int quads = hd / 4, halves = quads <= 32 ? 2 : 1;      // (heads of up to 128: two parts at a time, 32 lanes each)
@@ -699,15 +754,17 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __rest
 template <typename T, int HD, int RB, int KS, int KT, int NS>
 static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
                        int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
-                       const int32_t* positions, const TreeSizes& z, int n_seqs, int nkv, int group, int max_q_len, int parts, int chunk, hipStream_t s) {
+                       const int32_t* positions, const TreeSizes& z, int n_seqs, int nkv, int group, int max_q_len, int parts, int want, hipStream_t s) {
     constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS>();
     static_assert(lds <= 159 * 1024, "a CU's LDS");
-    if (chunk % (KT * KS) != 0 || parts > kMostParts) return EGPT_BAD_ARGUMENT;
-    // (no more works than this: blocks of rows of all tokens and one begun per request, and the most blocks of a request times the requests)
-    const long long rows = static_cast<long long>(z.n_tokens) * group, blocks = (max_q_len * group + 32 * RB - 1) / (32 * RB);
-    const long long works = (rows / (32 * RB) + n_seqs < blocks * n_seqs ? rows / (32 * RB) + n_seqs : blocks * n_seqs) * nkv * parts;
+    if (parts > kMostParts) return EGPT_BAD_ARGUMENT;
+    // No more blocks than this: of rows of all tokens and one begun per request, and the most of a request times the requests.  And no more works: `want`, or half a
+    // part a block beyond it where they do not come out even.
+    const long long rows = static_cast<long long>(z.n_tokens) * group, most = (max_q_len * group + 32 * RB - 1) / (32 * RB);
+    const long long blocks = (rows / (32 * RB) + n_seqs < most * n_seqs ? rows / (32 * RB) + n_seqs : most * n_seqs) * nkv;
+    const long long wanted = want > blocks ? want : blocks, works = parts > 1 ? wanted + blocks : blocks;
     const long long grid = (works + 7) / 8 * 8;
-    if (grid >= 1 << 27) return EGPT_UNSUPPORTED_SIZE;
+    if (grid >= 1 << 26) return EGPT_UNSUPPORTED_SIZE;
     auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
     if (lds > 60 * 1024) {                                   // more than a launch may have unasked: asked for once per instance and device
         static std::atomic<unsigned long long> raised{0};
@@ -719,14 +776,15 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
             raised.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, chunk, magic_of(chunk), group, max_q_len,
-                                                                   table_width, q_start, static_cast<const T*>(qkv), visible, positions,
+    int* const per = parts > 1 ? reinterpret_cast<int*>(part_ml + static_cast<size_t>(parts) * z.n_tokens * z.nq * 2) : nullptr;
+    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, static_cast<int>(wanted), group, max_q_len,
+                                                                   table_width, magic_of(parts), q_start, static_cast<const T*>(qkv), visible, positions,
                                                                    static_cast<const T*>(k_cache), static_cast<const T*>(v_cache), static_cast<T*>(out),
-                                                                   part_o, part_ml, z);
+                                                                   part_o, part_ml, per, z);
     EGPT_CHECK_LAUNCH();
     if (parts > 1) {
-        tree_combine_kernel<T><<<dim3((max_q_len * z.nq + 3) / 4, n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, chunk, magic_of(chunk), z.nq,
-                                                                                 magic_of(z.nq), max_q_len, parts, z.n_tokens, z.hd, static_cast<T*>(out));
+        tree_combine_kernel<T><<<dim3((max_q_len * z.nq + 3) / 4, n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, per, KT * KS, z.nq,
+                                                                                 magic_of(z.nq), max_q_len, z.n_tokens, z.hd, static_cast<T*>(out));
         EGPT_CHECK_LAUNCH();
     }
     return EGPT_OK;
@@ -763,11 +821,11 @@ extern "C" int egpt_tree_attention_generic(const void* qkv, void* out, const voi
 extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache,
                                    const int32_t* block_table, int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len,
                                    const int32_t* kv_len, const long long* visible, const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv,
-                                   int hd, int page_size, float scale, int window, int max_q_len, int shape, int parts, int chunk, int dtype, void* stream) {
+                                   int hd, int page_size, float scale, int window, int max_q_len, int shape, int parts, int want, int dtype, void* stream) {
     if (!qkv || !out || !k_cache || !v_cache || !block_table || !q_start || !q_len || !kv_len || !visible || (window > 0 && !positions))
         return EGPT_BAD_ARGUMENT;
     if (n_seqs <= 0 || n_tokens < 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || hd <= 0 || page_size <= 0 || table_width <= 0 || window < 0 ||
-        n_pages < 0 || max_q_len < 0 || dtype < 0 || dtype > 1 || parts <= 0 || chunk <= 0 || (parts > 1 && (!part_o || !part_ml)))
+        n_pages < 0 || max_q_len < 0 || dtype < 0 || dtype > 1 || parts <= 0 || want <= 0 || (parts > 1 && (!part_o || !part_ml)))
         return EGPT_BAD_ARGUMENT;
     const int size = dtype == 0 ? 4 : 2;
     if (hd > kMaxTreeHead || hd * size % 16 != 0 || page_size % kGroup != 0 || max_q_len > 64 || nq > 65535 || n_seqs > 65535 ||
@@ -780,7 +838,7 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
     const TreeSizes z{n_pages, page_size, nq, hd, window, n_tokens, magic_of(group), magic_of(page_size), scale};
 #define EGPT_TREE(...) \
     return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, table_width, q_start, q_len, kv_len, visible, positions, z, n_seqs, nkv, \
-                                    group, max_q_len, parts, chunk, static_cast<hipStream_t>(stream))
+                                    group, max_q_len, parts, want, static_cast<hipStream_t>(stream))
     // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS)
     if (dtype == 1 && hd <= 64) {
         if (shape == 14) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);

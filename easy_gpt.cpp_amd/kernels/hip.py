@@ -2292,13 +2292,13 @@ class HipKernels(KernelBackend):
         more = (block_table.data_ptr(), width, pages, q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
                 positions.data_ptr() if window else None, b, t, nq, nkv, hd, page_size, float(scale), int(window))
         if hd * (4 if dt == 0 else 2) % 16 == 0 and page_size % 16 == 0 and not (at_q | at_out | at_k | at_v) & 15:
-            shape, parts, chunk = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 64) * 64)
+            shape, parts, want = self._tree_shape(b, t, nkv, nq // nkv, hd, dt, max_q_len, -(-max_kv_len // 64) * 64)
             part_o = part_ml = None
             if parts > 1:
                 rows = parts * t * nq
-                part_o = torch.empty(rows * (hd + 2), dtype=_F32, device=qkv.device)
+                part_o = torch.empty(rows * (hd + 2) + 1, dtype=_F32, device=qkv.device)
                 part_ml = part_o.data_ptr() + 4 * rows * hd
-            self._run("egpt_tree_attention", at_q, at_out, self._ptr(part_o), part_ml, at_k, at_v, *more, int(max_q_len), shape, parts, chunk, dt,
+            self._run("egpt_tree_attention", at_q, at_out, self._ptr(part_o), part_ml, at_k, at_v, *more, int(max_q_len), shape, parts, want, dt,
                       self._stream())
             return
         self._run("egpt_tree_attention_generic", at_q, at_out, at_k, at_v, *more, dt, self._stream())
@@ -2306,28 +2306,28 @@ class HipKernels(KernelBackend):
     # The matrix-core kernel for trees by type (0 float32) and head size: its shapes (10 * blocks of 32 rows to a workgroup + wavefronts that share a
     # block's keys), keys of a round, workgroups that a CU holds, and a fit of what was measured (50 sizes of 1 to 64 requests, 1 to 64 nodes,
     # 128 to 32,000 tokens before them, in up to 64 parts): microseconds before the first round, of a round with one workgroup to a CU and with as
-    # many as it holds.  (By the fit's choice 3 % slower than the best of what was measured; 64 requests of 1 to 32 nodes behind 128 to 4,000 tokens 17 %,
-    # whose sums it cannot know.)
+    # many as it holds.  (By the fit's choice 0.5 % slower than the best of what was measured, 6 % at most.)
     _tree_shapes = {
-        (1, 64): ((14, 128, 2, 5.4, 0.77, 1.27), (22, 128, 2, 5.44, 1.04, 1.66), (41, 64, 3, 5.21, 0.93, 1.13)),
-        (1, 128): ((14, 128, 1, 5.84, 1.44, 1.44), (22, 64, 2, 6.43, 1.04, 1.42), (81, 64, 1, 6.09, 1.91, 1.91)),
+        (1, 64): ((14, 128, 2, 5.49, 0.8, 1.22), (22, 128, 2, 5.49, 1.07, 1.61), (41, 64, 3, 5.45, 0.89, 1.16)),
+        (1, 128): ((14, 128, 1, 5.97, 1.46, 1.46), (22, 64, 2, 6.58, 1.05, 1.29), (81, 64, 1, 6.41, 1.93, 1.93)),
         (1, 256): ((12, 64, 1, 6.95, 2.25, 2.25), (41, 32, 1, 5.7, 2.08, 2.08)),
-        (0, 64): ((14, 128, 1, 4.7, 3.35, 3.35), (22, 64, 2, 6.51, 2.41, 4.75)),
-        (0, 128): ((22, 64, 1, 7.23, 4.85, 4.85), (41, 32, 2, 7.08, 4.06, 9.84)),
+        (0, 64): ((14, 128, 1, 5.28, 3.36, 3.36), (22, 64, 2, 6.75, 2.29, 4.33)),
+        (0, 128): ((22, 64, 1, 7.89, 4.91, 4.91), (41, 32, 2, 7.39, 4.26, 9.74)),
         (0, 256): ((41, 32, 1, 7.0, 8.0, 8.0),),
     }
 
     @classmethod
     @functools.lru_cache(maxsize=4096)
     def _tree_shape(cls, b, t, nkv, group, hd, dt, max_q_len, max_kv_len) -> tuple[int, int, int]:
-        """(shape, parts of a request's keys at most, keys of a part) of the matrix-core kernel for trees: the cheapest by the fit.  The joining
-        kernel costs 3 us and 0.26 for a megabyte of the parts' results."""
-        best = None
+        """(shape, parts of a request's keys at most, workgroups in all) of the matrix-core kernel for trees: the cheapest by the fit for requests that all
+        have the longest context; the kernel cuts those that there are into as many.  The joining
+        kernel costs 3.2 us and 0.28 for a megabyte of the parts' results."""
+        best, rounds_of = None, {}
         for shape, keys, held, launch, alone, full in cls._tree_shapes[dt, 64 if hd <= 64 else 128 if hd <= 128 else 256]:
             rows = 32 * (shape // 10)
             blocks = min(-(-max_q_len * group // rows) * b, t * group // rows + b) * nkv
-            rounds = last = -(-max_kv_len // keys)
-            for wanted in (1, 2, 3, 4, 6, 8, 11, 16, 22, 32, 48, 64):
+            rounds = last = rounds_of[shape] = -(-max_kv_len // keys)
+            for wanted in sorted({1, 2, 3, 4, 6, 8, 11, 16, 22, 32, 48, 64} | {min(64, 256 * h // blocks) for h in range(1, held + 1) if 256 * h >= blocks}):
                 per = max(-(-rounds // wanted), 1)                   # rounds of a part
                 parts = -(-rounds // per)
                 if parts == last and wanted > 1:
@@ -2335,12 +2335,16 @@ class HipKernels(KernelBackend):
                 last = parts
                 works = blocks * parts
                 turns = max(1, -(-works // (256 * held)))
-                us = launch + turns * per * (alone + (full - alone) * min(1.0, max(0.0, works / turns / 256 - 1) / max(held - 1, 1))) + (turns - 1) * 1.5
+                beside = max(1, -(-works // (256 * turns)))          # workgroups of a CU at a time
+                us = launch + turns * per * (alone + (full - alone) * (beside - 1) / max(held - 1, 1)) + (turns - 1) * 1.5
                 if parts > 1:
-                    us += 3.0 + 0.26e-6 * parts * t * group * nkv * hd * 8
+                    us += 3.2 + 0.28e-6 * parts * t * group * nkv * hd * 8
                 if best is None or us < best[0]:
-                    best = us, shape, parts, per * keys
-        return best[1:]
+                    best = us, shape, parts, works
+        us, shape, parts, works = best
+        if parts > 1 and b > 1:                              # (room for the long ones of uneven contexts to have more parts, up to 256 MB of results)
+            parts = max(parts, min(64, rounds_of[shape], 3 * parts, (64 << 20) // (t * group * nkv * hd)))
+        return shape, parts, works
 
     def accept_drafts(self, tokens, parents, sampled, q_start, q_len):
         t, b = tokens.numel(), q_len.numel()

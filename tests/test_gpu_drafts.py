@@ -179,6 +179,26 @@ def test_many_ragged_requests(dtype):
     check_tree(c)
 
 
+@pytest.mark.parametrize("loose", [False, True], ids=["bounds", "loose_bounds"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (6, 1, 128), (4, 1, 256)], ids=str)
+def test_uneven_contexts_are_cut_by_what_they_are(heads, loose):
+    # one long context beside short and empty ones, in more requests than a wavefront has lanes and in few: parts of every length; and bounds far
+    # above what there is, as a captured step has them
+    rng = random.Random(21)
+    for b in (2, 5, 131):
+        lens = [rng.choice([0, 1, 2, 5, 11]) for _ in range(b)]
+        befores = [rng.choice([0, 1, 15, 64, 127, 300]) for _ in range(b)]
+        lens[b // 2], befores[b // 2] = 13, 1777
+        lens[-1], befores[-1] = 3, 640
+        c, _ = plain.tree_case(rng, lens, befores, *heads, 16, BF16, DEV)
+        if loose:
+            c["block_table"] = torch.cat([c["block_table"], torch.full((b, 200), -1, dtype=torch.int32, device=DEV)], 1)
+        out = torch.full((c["qkv"].shape[0], c["nq"] * c["hd"]), math.nan, dtype=BF16, device=DEV)
+        kernels.backend().tree_attention(c["qkv"], out, c["k_cache"], c["v_cache"], c["block_table"], c["q_start"], c["q_len"], c["kv_len"], c["visible"],
+                                         *heads, 16, c["scale"], 64 if loose else 13, c["block_table"].shape[1] * 16 if loose else int(c["kv_len"].max()))
+        check_tree(c, out)
+
+
 def test_a_chain_is_a_prompt_portion():
     # every node sees all before it: what paged_attention does with those tokens
     c, _ = plain.tree_case(random.Random(14), [40, 12], [130, 6], 6, 2, 64, 16, BF16, DEV, parents=[list(range(-1, 39)), list(range(-1, 11))])
