@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
 //
 // Tiles go from memory straight to LDS, NS - 1 of them ahead of their use, one barrier a tile.  A load takes 1,024 bytes that lie in one page: a
 // resource with that page's base, bounded by it, and a constant offset per lane.  Keys lie in rows, 16-byte pieces exchanged by the row's number, values as a page of 16
-// tokens has them: either way 64 lanes read different banks.  A head that is no power of two is filled up with zeros by the loads' bounds.
+// tokens has them, halves exchanged by the feature's: either way lanes that read together read different banks.  A head that is no power of two is filled up with zeros by the loads' bounds.
 //
 // A request's keys are cut into parts, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
 // parts leave the unnormalised result with its maximum and sum, and tree_combine_kernel joins them.
@@ -342,11 +342,13 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     const char* const v_head = reinterpret_cast<const char*>(v_cache) + kvh * head_bytes;
     // A wavefront's loads of a tile: EACH of a group's PER_GROUP, of OWN groups.  Load u has the group's keys from u * (1024 / ROWB) on, and the values' features from
     // u * (64 / SZ) on; what differs between a wavefront's loads is a scalar offset and, in the exchange of a key's pieces, bits of its number above the lane's.
-    constexpr int row_swap = PIECES >= 16 ? 15 : 7, KEYS = 1024 / ROWB;
+    constexpr int KEYS = 1024 / ROWB;
     const int first_load = rb * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
-    auto swap_of = [](int key) { return (SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key) & row_swap; };      // bfloat16: bits 2 and 3 exchanged
+    // (16 lanes read 256 bytes, all banks, at a time: their rows' pieces lie in 16 different places, two rows of 128 bytes side by side)
+    auto swap_at = [](int lane_row) { return PIECES >= 16 ? lane_row & 15 : lane_row >> 1 & 7; };
+    auto swap_of = [&](int key) { return swap_at(SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key); };      // bfloat16: bits 2 and 3 exchanged
     const int k_at = lane / PIECES * key_bytes, k_place = lane % PIECES ^ swap_of(lane / PIECES);
-    const int v_at = lane / SZ * z.page_size * SZ + (SZ == 2 ? lane % 2 : (lane % 4) ^ (lane / SZ >> 2 & 3)) * 16;       // (features past the head's lie past the resource's end)
+    const int v_at = lane / SZ * z.page_size * SZ + (SZ == 2 ? lane % 2 ^ (lane >> 4 & 1) : (lane % 4) ^ (lane / SZ >> 2 & 3)) * 16;       // (features past the head's lie past the resource's end)
     const int n_tiles = (groups * kGroup + KT - 1) / KT, rounds = (n_tiles + KS - 1) / KS;
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)smem));
     // (`places`: those of the 64 groups that the round's keys are among)
@@ -427,8 +429,8 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     float m_run = -INFINITY, l_run = 0.f;
     const float scale2 = fabsf(z.scale) * 1.4426950408889634f;   // exponentials are taken to the base 2
     const int my_key = SZ == 2 ? (lr & 3) | (lr >> 1 & 4) | (lr << 1 & 8) | (lr & 16) : lr;
-    const int k_row = my_key * ROWB, k_piece = (lh ^ (lr & row_swap)) * 16;
-    const int v_row = lr * kGroup * SZ + (SZ == 2 ? lh * 16 : ((lh ^ (lr >> 2 & 3)) * 16));
+    const int k_row = my_key * ROWB, k_piece = (lh ^ swap_at(lr)) * 16;
+    const int v_row = lr * kGroup * SZ + (SZ == 2 ? (lh ^ (lr >> 3 & 1)) * 16 : ((lh ^ (lr >> 2 & 3)) * 16));
 
     auto piece_at = [&](const char* at) { return *reinterpret_cast<const u32x4*>(at); };
     auto values_at = [&](const char* tile, int kb, int step, int d) {
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
                 for (int e = 0; e < 16; ++e) {
                     const int feature = d * 32 + e / 4 * 8 + lh * 4 + e % 4, in = key % kGroup;
                     float v;
-                    if constexpr (SZ == 2) v = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(values + feature * 32 + in * 2)) << 16);
+                    if constexpr (SZ == 2) v = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(values + feature * 32 + ((in / 8) ^ (feature >> 3 & 1)) * 16 + in % 8 * 2)) << 16);
                     else v = *reinterpret_cast<const float*>(values + feature * 64 + ((in / 4) ^ (feature >> 2 & 3)) * 16 + in % 4 * 4);
                     const float scaled = acc[d][e] * alpha;
                     acc[d][e] = sees ? fmaf(w, v, scaled) : scaled;
