@@ -10,7 +10,8 @@ prompt portions in arrival order.
 
 With drafts (`SchedulerConfig.draft_nodes`) a step in which every entry decodes checks, beside each request's last token, what its
 own tokens say may follow (`engine.drafting`), and a request may gain several tokens from it; the tokens are those that it would
-have without, since the uniform number of its n-th token is the same either way.  Steps then wait for each other.
+have without, since the uniform number of its n-th token is the same either way (bfloat16 rounds the logits of a step with more rows
+otherwise, as for any batch).  Steps then wait for each other.
 
 Decoding runs one step ahead of the host where it can: while a decode step is on the GPU, the next one (the same
 requests, one token each) is launched behind it with its token ids taken on the device from what the sampler leaves
