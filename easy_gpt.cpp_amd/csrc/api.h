@@ -418,8 +418,8 @@ int egpt_tree_attention_generic(const void* qkv, void* out, const void* k_cache,
 // <= 64 nodes.  A request's keys are cut into at most `parts` <= 64 parts, so many that there are about `want`
 // workgroups; with parts > 1, part_o [parts][n_tokens][nq][hd] and part_ml [parts][n_tokens][nq][2] (float32) and one int behind the latter hold
 // their results until a second kernel joins them.  shape: 10 * blocks
-// of 32 rows that a workgroup takes + wavefronts that share a block's keys: bfloat16 up to head size 64 14, 22, 41, up to 128 14, 22, 81, beyond 12, 41;
-// float32 14, 22; 22, 41; 41.
+// of 32 rows that a workgroup takes + wavefronts that share a block's keys: bfloat16 up to head size 64 14, 22, 41, up to 128 14, 22, 81, beyond 11, 21, 41;
+// float32 14, 22; 22, 41; 21.
 int egpt_tree_attention(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
                         int table_width, int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
                         const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,

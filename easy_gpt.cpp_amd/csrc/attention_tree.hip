@@ -143,6 +143,10 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
 // resource with that page's base, bounded by it, and a constant offset per lane.  Keys lie in rows, 16-byte pieces exchanged by the row's number, values as a page of 16
 // tokens has them, halves exchanged by the feature's: either way lanes that read together read different banks.  A head that is no power of two is filled up with zeros by the loads' bounds.
 //
+// A head beyond 128 is more registers of queries and sums than a wavefront has: two share a block of rows, each with half of the features, and add up their halves of
+// the scores through LDS, one barrier more a tile (float32, 7 requests of one node behind 1,246 tokens at 12 heads on 2 of 256: 71.6 us by one wavefront with its
+// registers in memory, 29.0 so, and half the rounding error).
+//
 // A request's keys are cut into parts, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
 // parts leave the unnormalised result with its maximum and sum, and tree_combine_kernel joins them.
 typedef __attribute__((ext_vector_type(8))) __bf16 tree_bf16x8;
@@ -181,10 +185,11 @@ struct TreeSizes {
     float scale;
 };
 
-template <typename T, int HD, int RB, int KS, int KT, int NS>
+template <typename T, int HD, int RB, int KS, int KT, int NS, int FS>
 constexpr int tree_lds() {
     constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = KS * RB * 64 * (HD / 2 + 2) * 4;
-    return KS == 1 || stages > join ? stages : join;
+    constexpr int given = FS > 1 ? RB * FS * (KT / 32) * 16 * 64 * 4 : 0;      // the halves of the scores, behind the tiles
+    return (KS == 1 || stages > join ? stages : join) + given;
 }
 
 // The rounds of `keys` (a power of two) keys that a context takes, one at least; contexts are below 2^27.
@@ -289,8 +294,8 @@ __device__ __forceinline__ bool find_work(const int32_t* __restrict__ q_len, con
 }
 
 // (the first 14 words of the arguments arrive with the wavefronts: all that the first trip to memory needs)
-template <typename T, int HD, int RB, int KS, int KT, int NS>
-__global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1) void tree_attention_kernel(
+template <typename T, int HD, int RB, int KS, int KT, int NS, int FS>
+__global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T)) <= 256 || RB * FS > 4 ? 2 : 1) void tree_attention_kernel(
     const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ block_table, int n_seqs, int nkv, int most_parts,
     int want, int group, int max_q_len, int table_width, unsigned magic_most, const int32_t* __restrict__ q_start,
     const T* __restrict__ qkv, const long long* __restrict__ visible, const int32_t* __restrict__ positions, const T* __restrict__ k_cache,
@@ -298,15 +303,17 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     constexpr int SZ = sizeof(T);
     constexpr int ROWB = HD * SZ, PIECES = ROWB / 16, KC = ROWB / 32, DB = HD / 32, KB = KT / 32;
     constexpr int HALF = KT * ROWB, TILE = 2 * HALF;             // bytes of a tile's keys, and of it all
-    constexpr int LOADS = HALF / 1024 / RB;                      // of a wavefront and tile, keys and values each
+    constexpr int KC_OWN = KC / FS, DB_OWN = DB / FS;            // pieces of 32 bytes of a key, blocks of 32 features of a value: a wavefront's
+    constexpr int LOADS = HALF / 1024 / (RB * FS);               // of a wavefront and tile, keys and values each
     constexpr int PER_GROUP = ROWB / 64;                         // loads of a group of 16 keys
     constexpr int OWN = LOADS > PER_GROUP ? LOADS / PER_GROUP : 1, EACH = LOADS > PER_GROUP ? PER_GROUP : LOADS;
     constexpr int STEPS = SZ == 2 ? 2 : 4;                       // second products of a block of 32 keys: 32 bytes of a feature each
-    static_assert(LOADS >= 1 && HALF % (1024 * RB) == 0 && OWN * EACH == LOADS, "every wavefront loads as much");
+    static_assert(FS == 1 || KS == 1, "wavefronts that share features have the same keys");
+    static_assert(LOADS >= 1 && HALF % (1024 * RB * FS) == 0 && OWN * EACH == LOADS, "every wavefront loads as much");
     static_assert(kWave * kGroup % (KT * KS) == 0, "the 64 groups that a wavefront has the pages of are whole rounds");
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 32, lh = lane / 32;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), rb = wave % RB, ksi = wave / RB;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), rb = wave % RB, fs = wave / RB % FS, ksi = wave / (RB * FS);
 
     // which part of which request and kv head, and which block of its rows
     auto blocks_of = [&](int n_) { return (min(max(n_, 0), max_q_len) * group + 32 * RB - 1) / (32 * RB); };
@@ -343,7 +350,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     // A wavefront's loads of a tile: EACH of a group's PER_GROUP, of OWN groups.  Load u has the group's keys from u * (1024 / ROWB) on, and the values' features from
     // u * (64 / SZ) on; what differs between a wavefront's loads is a scalar offset and, in the exchange of a key's pieces, bits of its number above the lane's.
     constexpr int KEYS = 1024 / ROWB;
-    const int first_load = rb * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
+    const int first_load = (fs * RB + rb) * LOADS, group_first = first_load / PER_GROUP, load_first = first_load % PER_GROUP;
     // (16 lanes read 256 bytes, all banks, at a time: their rows' pieces lie in 16 different places, two rows of 128 bytes side by side)
     auto swap_at = [](int lane_row) { return PIECES >= 16 ? lane_row & 15 : lane_row >> 1 & 7; };
     auto swap_of = [&](int key) { return swap_at(SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key); };      // bfloat16: bits 2 and 3 exchanged
@@ -410,20 +417,20 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
         if (first_round + i < rounds) load_round(first_round + i);
 
     const unsigned long long bits = valid ? static_cast<unsigned long long>(visible[token]) : 0ull;
-    u32x4 q[KC];
-    {
-        const char* qp = reinterpret_cast<const char*>(qkv + static_cast<size_t>(token) * (z.nq + 2 * nkv) * z.hd + head * z.hd);
+    const char* const q_row = reinterpret_cast<const char*>(qkv + static_cast<size_t>(token) * (z.nq + 2 * nkv) * z.hd + head * z.hd);
+    auto query_at = [&](int i) {
+        const int at = i * 32 + lh * 16;
+        u32x4 one = valid && at < key_bytes ? *reinterpret_cast<const u32x4*>(q_row + at) : u32x4{0u, 0u, 0u, 0u};
+        if (z.scale < 0.f) one ^= SZ == 2 ? 0x80008000u : 0x80000000u;             // (the greatest score is the greatest product then as well)
+        return one;
+    };
+    u32x4 q[KC_OWN];
 #pragma unroll
-        for (int i = 0; i < KC; ++i) {
-            const int at = i * 32 + lh * 16;
-            q[i] = valid && at < key_bytes ? *reinterpret_cast<const u32x4*>(qp + at) : u32x4{0u, 0u, 0u, 0u};
-            if (z.scale < 0.f) q[i] ^= SZ == 2 ? 0x80008000u : 0x80000000u;        // (the greatest score is the greatest product then as well)
-        }
-    }
+    for (int i = 0; i < KC_OWN; ++i) q[i] = query_at(fs * KC_OWN + i);
 
-    f32x16 acc[DB];
+    f32x16 acc[DB_OWN];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB_OWN; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
@@ -436,7 +443,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     auto values_at = [&](const char* tile, int kb, int step, int d) {
         const int g = kb * 2 + (SZ == 2 ? step : step / 2);
         const int row = SZ == 2 ? v_row : v_row ^ ((step % 2) * 32);
-        return piece_at(tile + HALF + (g * HD + d * 32) * kGroup * SZ + row);
+        return piece_at(tile + HALF + (g * HD + (fs * DB_OWN + d) * 32) * kGroup * SZ + row);
     };
     // A tile with values that are no finite numbers, some of them of nodes that not every row sees: a row's weight for such a key is zero, and zero times
     // an infinity is none.  So one key after the other, on the vector pipe, left out where it is not seen.  (Rare, and slow: registers that it held would be the other tiles'.)
@@ -449,18 +456,24 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             const bool sees = valid && (j < before ? j >= lo : j - before < 64 && (bits >> (j - before) & 1ull) != 0);
             if (!__any(sees)) continue;
             float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < KC; ++i) {
+            auto add = [&](int i, u32x4 query) {
                 const u32x4 k = *reinterpret_cast<const u32x4*>(tile + key * ROWB + (((2 * i + lh) ^ swap_of(key)) * 16));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (SZ == 2) {
-                        dot = fmaf(__uint_as_float(k[e] << 16), __uint_as_float(q[i][e] << 16), dot);
-                        dot = fmaf(__uint_as_float(k[e] & 0xffff0000u), __uint_as_float(q[i][e] & 0xffff0000u), dot);
+                        dot = fmaf(__uint_as_float(k[e] << 16), __uint_as_float(query[e] << 16), dot);
+                        dot = fmaf(__uint_as_float(k[e] & 0xffff0000u), __uint_as_float(query[e] & 0xffff0000u), dot);
                     } else {
-                        dot = fmaf(__uint_as_float(k[e]), __uint_as_float(q[i][e]), dot);
+                        dot = fmaf(__uint_as_float(k[e]), __uint_as_float(query[e]), dot);
                     }
                 }
+            };
+            if constexpr (FS > 1) {                                             // (the others' features as well, from memory)
+#pragma unroll 1
+                for (int i = 0; i < KC; ++i) add(i, query_at(i));
+            } else {
+#pragma unroll
+                for (int i = 0; i < KC; ++i) add(i, q[i]);
             }
             dot = fold_32_apart(dot, AddOf());
             const float m_new = sees ? fmaxf(m_run, dot) : m_run, m_use = m_new == -INFINITY ? 0.f : m_new;
@@ -469,11 +482,11 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             l_run = l_run * alpha + (sees && lh == 0 ? w : 0.f);             // (the halves' sums are added up in the end)
             const char* const values = tile + HALF + key / kGroup * HD * kGroup * SZ;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
+            for (int d = 0; d < DB_OWN; ++d) {
                 asm volatile("" ::: "memory");                                // (not all of them at once)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int feature = d * 32 + e / 4 * 8 + lh * 4 + e % 4, in = key % kGroup;
+                    const int feature = (fs * DB_OWN + d) * 32 + e / 4 * 8 + lh * 4 + e % 4, in = key % kGroup;
                     float v;
                     if constexpr (SZ == 2) v = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(values + feature * 32 + ((in / 8) ^ (feature >> 3 & 1)) * 16 + in % 8 * 2)) << 16);
                     else v = *reinterpret_cast<const float*>(values + feature * 64 + ((in / 4) ^ (feature >> 2 & 3)) * 16 + in % 4 * 4);
@@ -497,11 +510,13 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 #pragma unroll
                 for (int step = 0; step < STEPS; ++step)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) probe = product_of<T>(values_at(tile, kb, step, d), u32x4{0u, 0u, 0u, 0u}, probe);
+                    for (int d = 0; d < DB_OWN; ++d) probe = product_of<T>(values_at(tile, kb, step, d), u32x4{0u, 0u, 0u, 0u}, probe);
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) sum += probe[e];
-            if (__builtin_expect(__any(sum != 0.f), 0)) return strange_tile(tile, key0, places);
+            bool strange = __any(sum != 0.f) != 0;
+            if constexpr (FS > 1) strange = __syncthreads_or(strange) != 0;     // (the wavefronts of a row go the same way)
+            if (__builtin_expect(strange, 0)) return strange_tile(tile, key0, places);
         }
         f32x16 s[KB];
         unsigned sees[KB];
@@ -510,7 +525,32 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < KC; ++i) s[kb] = product_of<T>(piece_at(tile + kb * 32 * ROWB + k_row + (k_piece ^ (i * 32))), q[i], s[kb]);
+            for (int i = 0; i < KC_OWN; ++i)
+                s[kb] = product_of<T>(piece_at(tile + kb * 32 * ROWB + k_row + fs * KC_OWN * 32 + (k_piece ^ (i * 32))), q[i], s[kb]);
+        }
+        if constexpr (FS > 1) {                          // the scores of the other features, from the wavefronts that have them
+            tree_f32x4* const given = reinterpret_cast<tree_f32x4*>(smem + NS * KS * TILE) + lane;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    given[((wave * KB + kb) * 4 + e) * kWave] = tree_f32x4{s[kb][4 * e], s[kb][4 * e + 1], s[kb][4 * e + 2], s[kb][4 * e + 3]};
+            __syncthreads();
+#pragma unroll
+            for (int f = 1; f < FS; ++f) {
+                const int other = (fs + f) % FS * RB + rb;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const tree_f32x4 one = given[((other * KB + kb) * 4 + e) * kWave];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kb][4 * e + i] += one[i];
+                    }
+            }
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
             if constexpr (MASKED) {
                 const int k0 = key0 + kb * 32, cut = before - k0;               // keys of the block before the tree
                 unsigned long long w = cut >= 0 ? (cut < 32 ? bits << cut : 0ull) : (cut > -64 ? bits >> -cut : 0ull);
@@ -546,7 +586,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             l_run *= alpha;
             m_run = m_new;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DB_OWN; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
         }
@@ -580,7 +620,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
             for (int step = 0; step < STEPS; ++step) {
                 const u32x4 p = weights_of(kb, step);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = product_of<T>(values_at(tile, kb, step, d), p, acc[d]);
+                for (int d = 0; d < DB_OWN; ++d) acc[d] = product_of<T>(values_at(tile, kb, step, d), p, acc[d]);
             }
     };
 
@@ -630,10 +670,10 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
     // its share of the quads (one wavefront that joins them all is as long alone as two tiles: an instruction of a wavefront that has its SIMD to itself is 5 cycles).
     const size_t row = static_cast<size_t>(token) * z.nq + head, mine = static_cast<size_t>(part) * z.n_tokens * z.nq + row;
     const bool whole = n_parts == 1;
-    constexpr int QUADS = DB * 4, SHARE = QUADS / KS;
+    constexpr int QUADS = DB_OWN * 4, SHARE = QUADS / KS;
     static_assert(QUADS % KS == 0, "as many quads for every group");
     auto leave = [&](const float (&v)[4], int quad, float factor) {
-        const int at = quad / 4 * 32 + quad % 4 * 8 + lh * 4;
+        const int at = (fs * DB_OWN + quad / 4) * 32 + quad % 4 * 8 + lh * 4;
         const float o[4] = {v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor};
         if (at >= z.hd) return;
         if (whole) write_quad(out + row * z.hd + at, o);
@@ -645,7 +685,7 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
         float2* const sums = reinterpret_cast<float2*>(smem + KS * RB * QUADS * kWave * 16) + rb * kWave + lane;                  // [group][rb][lane]
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB_OWN; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 results[(ksi * RB * QUADS + d * 4 + e) * kWave] = tree_f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
@@ -685,14 +725,14 @@ __global__ __launch_bounds__(64 * RB * KS, HD * static_cast<int>(sizeof(T)) <= 2
         if (!valid) return;
         const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB_OWN; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float v[4] = {acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
                 leave(v, d * 4 + e, inv);
             }
     }
-    if (!whole && lh == 0 && ksi == 0) {
+    if (!whole && lh == 0 && ksi == 0 && fs == 0) {
         part_ml[mine * 2] = m_all * scale2;
         part_ml[mine * 2 + 1] = l;
     }
@@ -753,11 +793,11 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __rest
     write_quad(out + row * hd + at, o);
 }
 
-template <typename T, int HD, int RB, int KS, int KT, int NS>
+template <typename T, int HD, int RB, int KS, int KT, int NS, int FS = 1>
 static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml, const void* k_cache, const void* v_cache, const int32_t* block_table,
                        int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
                        const int32_t* positions, const TreeSizes& z, int n_seqs, int nkv, int group, int max_q_len, int parts, int want, hipStream_t s) {
-    constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS>();
+    constexpr int lds = tree_lds<T, HD, RB, KS, KT, NS, FS>();
     static_assert(lds <= 159 * 1024, "a CU's LDS");
     if (parts > kMostParts) return EGPT_BAD_ARGUMENT;
     // No more blocks than this: of rows of all tokens and one begun per request, and the most of a request times the requests.  And no more works: `want`, or half a
@@ -767,7 +807,7 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
     const long long wanted = want > blocks ? want : blocks, works = parts > 1 ? wanted + blocks : blocks;
     const long long grid = (works + 7) / 8 * 8;
     if (grid >= 1 << 26) return EGPT_UNSUPPORTED_SIZE;
-    auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS>;
+    auto kernel = tree_attention_kernel<T, HD, RB, KS, KT, NS, FS>;
     if (lds > 60 * 1024) {                                   // more than a launch may have unasked: asked for once per instance and device
         static std::atomic<unsigned long long> raised{0};
         int device = -1;
@@ -779,7 +819,7 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
         }
     }
     int* const per = parts > 1 ? reinterpret_cast<int*>(part_ml + static_cast<size_t>(parts) * z.n_tokens * z.nq * 2) : nullptr;
-    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, static_cast<int>(wanted), group, max_q_len,
+    kernel<<<static_cast<unsigned>(grid), 64 * RB * KS * FS, lds, s>>>(q_len, kv_len, block_table, n_seqs, nkv, parts, static_cast<int>(wanted), group, max_q_len,
                                                                    table_width, magic_of(parts), q_start, static_cast<const T*>(qkv), visible, positions,
                                                                    static_cast<const T*>(k_cache), static_cast<const T*>(v_cache), static_cast<T*>(out),
                                                                    part_o, part_ml, per, z);
@@ -841,7 +881,7 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
 #define EGPT_TREE(...) \
     return launch_tree<__VA_ARGS__>(qkv, out, part_o, part_ml, k_cache, v_cache, block_table, table_width, q_start, q_len, kv_len, visible, positions, z, n_seqs, nkv, \
                                     group, max_q_len, parts, want, static_cast<hipStream_t>(stream))
-    // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS)
+    // (type, head size, blocks of rows, groups of wavefronts, keys of a tile, tiles in LDS, wavefronts that share a block's features)
     if (dtype == 1 && hd <= 64) {
         if (shape == 14) EGPT_TREE(bf16_t, 64, 1, 4, 32, 2);
         if (shape == 22) EGPT_TREE(bf16_t, 64, 2, 2, 64, 2);
@@ -851,16 +891,17 @@ extern "C" int egpt_tree_attention(const void* qkv, void* out, float* part_o, fl
         if (shape == 22) EGPT_TREE(bf16_t, 128, 2, 2, 32, 2);
         if (shape == 81) EGPT_TREE(bf16_t, 128, 8, 1, 64, 3);
     } else if (dtype == 1) {
-        if (shape == 12) EGPT_TREE(bf16_t, 256, 1, 2, 32, 2);
-        if (shape == 41) EGPT_TREE(bf16_t, 256, 4, 1, 32, 3);
+        if (shape == 11) EGPT_TREE(bf16_t, 256, 1, 1, 32, 2, 2);
+        if (shape == 21) EGPT_TREE(bf16_t, 256, 2, 1, 32, 3, 2);
+        if (shape == 41) EGPT_TREE(bf16_t, 256, 4, 1, 32, 3, 2);
     } else if (hd <= 64) {
         if (shape == 14) EGPT_TREE(float, 64, 1, 4, 32, 2);
         if (shape == 22) EGPT_TREE(float, 64, 2, 2, 32, 2);
     } else if (hd <= 128) {
         if (shape == 22) EGPT_TREE(float, 128, 2, 2, 32, 2);
         if (shape == 41) EGPT_TREE(float, 128, 4, 1, 32, 2);
-    } else if (shape == 41) {
-        EGPT_TREE(float, 256, 4, 1, 32, 2);
+    } else if (shape == 21) {
+        EGPT_TREE(float, 256, 2, 1, 32, 2, 2);
     }
 #undef EGPT_TREE
     return EGPT_BAD_ARGUMENT;

@@ -2304,16 +2304,16 @@ class HipKernels(KernelBackend):
         self._run("egpt_tree_attention_generic", at_q, at_out, at_k, at_v, *more, dt, self._stream())
 
     # The matrix-core kernel for trees by type (0 float32) and head size: its shapes (10 * blocks of 32 rows to a workgroup + wavefronts that share a
-    # block's keys), keys of a round, workgroups that a CU holds, and a fit of what was measured (50 sizes of 1 to 64 requests, 1 to 64 nodes,
+    # block's keys), keys of a round, workgroups that a CU holds, and a fit of what was measured (62 sizes of 1 to 64 requests, 1 to 64 nodes,
     # 128 to 32,000 tokens before them, in up to 64 parts): microseconds before the first round, of a round with one workgroup to a CU and with as
-    # many as it holds.  (By the fit's choice 0.5 % slower than the best of what was measured, 6 % at most.)
+    # many as it holds.  (By the fit's choice 1 % slower than the best of what was measured, 8 % at most.)
     _tree_shapes = {
         (1, 64): ((14, 128, 2, 5.49, 0.8, 1.22), (22, 128, 2, 5.49, 1.07, 1.61), (41, 64, 3, 5.45, 0.89, 1.16)),
         (1, 128): ((14, 128, 1, 5.97, 1.46, 1.46), (22, 64, 2, 6.58, 1.05, 1.29), (81, 64, 1, 6.41, 1.93, 1.93)),
-        (1, 256): ((12, 64, 1, 6.95, 2.25, 2.25), (41, 32, 1, 5.7, 2.08, 2.08)),
+        (1, 256): ((11, 32, 2, 6.5, 1.17, 1.51), (21, 32, 1, 6.47, 1.35, 1.35), (41, 32, 1, 6.62, 1.54, 1.54)),
         (0, 64): ((14, 128, 1, 5.28, 3.36, 3.36), (22, 64, 2, 6.75, 2.29, 4.33)),
         (0, 128): ((22, 64, 1, 7.89, 4.91, 4.91), (41, 32, 2, 7.39, 4.26, 9.74)),
-        (0, 256): ((41, 32, 1, 7.0, 8.0, 8.0),),
+        (0, 256): ((21, 32, 1, 8.6, 5.0, 5.0),),
     }
 
     @classmethod
