@@ -10,8 +10,8 @@
 //
 // What bounds it: for many rows the one pass over the logits (1,024 rows of 32,768 with top-p and min-p: 30.2 us, 4.4 TB/s, where a copy reaches 5.1;
 // 254 by the kernels that count and list in passes of their own, with a workgroup's list of hundreds compared pair by pair); for a few the chain of a load, a
-// dozen barriers and a second launch (1 row of 151,936 7.6 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 20.4).
-// Rows without a usable bound: 64 of 151,936 with top-p alone 263 us, nearly flat ones 45.
+// dozen barriers and a second launch (1 row of 151,936 7.6 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 19.1).
+// Rows without a usable bound: 64 of 151,936 with top-p alone 263 us, a min_p of 10^-6 45.
 #include "api.h"
 #include "common.h"
 #include "sampling.h"
@@ -573,10 +573,18 @@ extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, 
     float* maxima = reinterpret_cast<float*>(at += whole_blocks(n * sizeof(PieceOfRow)));
     uint2* lists = reinterpret_cast<uint2*>(at + whole_blocks(n * kMostShares * 4));
     const dim3 grid(n_rows, pieces);
-    if (small)
-        sample_pieces_kernel<2><<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists);
-    else
-        sample_pieces_kernel<8><<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists);
+    auto launch = [&](auto kernel) {
+        kernel<<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists);
+    };
+    switch ((quads_of_piece + kSampleThreads - 1) / kSampleThreads) {       // (quads a thread)
+        case 1:
+        case 2: launch(sample_pieces_kernel<2>); break;
+        case 3: launch(sample_pieces_kernel<3>); break;
+        case 4: launch(sample_pieces_kernel<4>); break;
+        case 5: launch(sample_pieces_kernel<5>); break;
+        case 6: launch(sample_pieces_kernel<6>); break;
+        default: launch(sample_pieces_kernel<8>);
+    }
     EGPT_CHECK_LAUNCH();
     sample_joined_kernel<<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab, pieces, found, maxima, lists);
     EGPT_CHECK_LAUNCH();

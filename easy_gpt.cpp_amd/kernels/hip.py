@@ -2182,14 +2182,15 @@ class HipKernels(KernelBackend):
     @staticmethod
     def _sample_pieces(rows: int, vocab: int, aligned: bool) -> int:
         """How many pieces sampling with min-p makes of a row.  One workgroup takes a row that its registers hold, 32,768 tokens (three fewer where
-        rows begin between 16 bytes), by one launch; a longer row is of pieces of 8,192 as long as the device runs all of them at a time, two
-        workgroups a compute unit, beyond that of 32,768 (tokens of 151,936, us with 19 and with 5 pieces a row: 1 row 7.7 and 9.5, 16 rows 9.7 and
-        10.9, 32 rows 14.4 and 13.8, 256 rows 38 and 32; of 32,768 with 5 pieces and with 1: 1 row 9.4 and 8.2, 256 rows 19.3 and 11.7)."""
+        rows begin between 16 bytes), by one launch; a longer row is of pieces of 8,192 as long as those of all rows are about as many as there are
+        compute units, then of 20,480, and of 32,768 where there are many rows anyway (tokens of 151,936, us with 19, with 8 and with 5 pieces a
+        row: 1 row 7.6, 8.2 and 9.6, 32 rows 14.1, 12.1 and 14.0, 64 rows 15.9, 14.7 and 16.5, 1,024 rows 179, 130 and 126; of 32,768 with 5
+        pieces and with 1: 1 row 9.1 and 7.5, 256 rows 19.3 and 10.3)."""
         off = 0 if aligned else 3
         if vocab <= 32768 - off:
             return 1
-        small = -(-vocab // (8192 - off))
-        return small if rows * small <= 512 else -(-vocab // (32768 - off))
+        small, middling = -(-vocab // (8192 - off)), -(-vocab // (20480 - off))
+        return small if rows * small <= 320 else middling if rows * middling <= 2048 else -(-vocab // (32768 - off))
 
     @functools.lru_cache(maxsize=4096)
     def _sample_space(self, rows: int, pieces: int) -> int:
