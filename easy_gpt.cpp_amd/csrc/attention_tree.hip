@@ -738,56 +738,70 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
     }
 }
 
-// The parts of a request's keys joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A wavefront has as many rows as it has times hd / 4 lanes; lane p of each
-// (at most 64 parts) takes part p's maximum and sum, so that the weights of all are known after one trip, and the parts' sums come kAhead at a time.  A part
-// that saw nothing weighs nothing, whatever it holds.
-template <typename T>
+// The parts of a request's keys joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A row has L lanes, four features each, and a wavefront 64 / L rows; the
+// lanes take the parts' maxima and sums between them, so that the weights of all are known after one trip, and then the parts' sums, kAhead on their way at a time.  A
+// part that saw nothing weighs nothing, whatever it holds.  (64 uneven requests at heads of 64: a row to a
+// wavefront 8.8 us, four 5.6.)
+template <typename T, int L>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start,
                                                            const float* __restrict__ part_ml, const float* __restrict__ part_o, const int* __restrict__ per_of, int round_keys,
                                                            int nq, unsigned magic_heads, int nodes, int n_tokens, int hd, T* __restrict__ out) {
-    constexpr int kAhead = 8;
-    const int lane = threadIdx.x % kWave, w = blockIdx.x * 4 + threadIdx.x / kWave, b = blockIdx.y;
-    const int node = divided(w, nq, magic_heads), head = w - node * nq;
+    constexpr int kAhead = 8, ROWS = kWave / L, OWN = kMostParts / L;
+    __shared__ float s_weight[4 * ROWS][kMostParts];
+    const int lane = threadIdx.x % kWave, sub = lane % L, in = threadIdx.x / L, b = blockIdx.y;
+    const int w = blockIdx.x * 4 * ROWS + in, node = divided(w, nq, magic_heads), head = w - node * nq;
     const int n = q_len[b], kv = kv_len[b], token = q_start[b] + node;
-    const int per = *per_of, parts = upper_quotient(rounds_of_keys(kv, round_keys), per, __builtin_amdgcn_rcpf(static_cast<float>(per)));
-    if (node >= n || node >= nodes || parts < 2 || token < 0 || token >= n_tokens) return;
-    const size_t row = static_cast<size_t>(token) * nq + head, step = static_cast<size_t>(n_tokens) * nq;
-    const int quads = hd / 4, halves = quads <= 32 ? 2 : 1;      // (heads of up to 128: two parts at a time, 32 lanes each)
-    const int half = halves == 2 ? lane / 32 : 0, quad = halves == 2 ? lane % 32 : lane;
-    const int at = min(quad, quads - 1) * 4;
+    const int per = *per_of, parts = min(upper_quotient(rounds_of_keys(kv, round_keys), per, __builtin_amdgcn_rcpf(static_cast<float>(per))), kMostParts);
+    if (parts < 2) return;
+    const bool there = node < n && node < nodes && token >= 0 && token < n_tokens;
+    if (!__any(there)) return;
+    const size_t row = there ? static_cast<size_t>(token) * nq + head : 0, step = static_cast<size_t>(n_tokens) * nq;
+    const int quads = hd / 4, at = min(sub, quads - 1) * 4;
     const float* const from = part_o + row * hd + at;
     float v[kAhead][4];
     auto ask = [&](int p0) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) read_quad(from + min(p0 + i * halves + half, parts - 1) * step * hd, v[i]);
+        for (int i = 0; i < kAhead; ++i)
+            if (p0 + i < parts) read_quad(from + (p0 + i) * step * hd, v[i]);
     };
     ask(0);
-    const size_t mine = (min(lane, parts - 1) * step + row) * 2;
-    const float m = part_ml[mine], l = lane < parts ? part_ml[mine + 1] : 0.f;
-    const float m_most = wave_max(l != 0.f ? m : -INFINITY);
-    const float weight = l != 0.f ? __builtin_amdgcn_exp2f(m - m_most) : 0.f;
-    const float total = wave_sum(weight * l);
-    const unsigned long long some = __ballot(l != 0.f);
+    float m[OWN], l[OWN], most = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) {
+        const int p = sub + j * L;
+        const size_t mine = (min(p, parts - 1) * step + row) * 2;
+        if (j == 0 || j * L < parts) {
+            m[j] = part_ml[mine];
+            l[j] = p < parts ? part_ml[mine + 1] : 0.f;
+            most = fmaxf(most, l[j] != 0.f ? m[j] : -INFINITY);
+        }
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, kWave));
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) {
+        if (j > 0 && j * L >= parts) continue;
+        const float weight = l[j] != 0.f ? __builtin_amdgcn_exp2f(m[j] - most) : 0.f;
+        total = fmaf(weight, l[j], total);
+        s_weight[in][sub + j * L] = l[j] != 0.f ? weight : -1.f;      // (of a part that saw nothing, whose sums may be anything)
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) total += __shfl_xor(total, o, kWave);
+    __builtin_amdgcn_wave_barrier();                                   // (a row's weights are read by the wavefront that wrote them)
     float sum[4] = {};
     for (int p0 = 0;;) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int p = p0 + i * halves + half;
-            const float share = __shfl(weight, p % kWave, kWave);
-            if (p < parts && (some >> (p % kWave) & 1ull)) {
+            if (p0 + i >= parts) break;
+            const float share = s_weight[in][p0 + i];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[i][e], share, sum[e]);
-            }
+            for (int e = 0; e < 4; ++e) sum[e] = share == -1.f ? sum[e] : fmaf(v[i][e], share, sum[e]);
         }
-        p0 += kAhead * halves;
+        p0 += kAhead;
         if (p0 >= parts) break;
         ask(p0);
     }
-    if (halves == 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = fold_32_apart(sum[e], AddOf());
-    }
-    if (half != 0 || quad >= quads) return;
+    if (!there || sub >= quads) return;
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     const float o[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
     write_quad(out + row * hd + at, o);
@@ -825,8 +839,9 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
                                                                    part_o, part_ml, per, z);
     EGPT_CHECK_LAUNCH();
     if (parts > 1) {
-        tree_combine_kernel<T><<<dim3((max_q_len * z.nq + 3) / 4, n_seqs), 256, 0, s>>>(q_len, kv_len, q_start, part_ml, part_o, per, KT * KS, z.nq,
-                                                                                 magic_of(z.nq), max_q_len, z.n_tokens, z.hd, static_cast<T*>(out));
+        constexpr int L = HD <= 64 ? 16 : HD <= 128 ? 32 : 64, rows_of_group = 4 * (kWave / L);
+        tree_combine_kernel<T, L><<<dim3((max_q_len * z.nq + rows_of_group - 1) / rows_of_group, n_seqs), 256, 0, s>>>(
+            q_len, kv_len, q_start, part_ml, part_o, per, KT * KS, z.nq, magic_of(z.nq), max_q_len, z.n_tokens, z.hd, static_cast<T*>(out));
         EGPT_CHECK_LAUNCH();
     }
     return EGPT_OK;
