@@ -500,24 +500,6 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
     auto tile_of = [&](auto masked, const char* tile, int key0, const Places& places) {
         constexpr bool MASKED = decltype(masked)::value;
         constexpr int R = SZ == 2 ? 8 : 4;                                      // neighbouring keys of a lane
-        if constexpr (MASKED) {
-            // whether any value is no finite number: their products with zeros are zeros unless it is
-            f32x16 probe;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) probe[e] = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int step = 0; step < STEPS; ++step)
-#pragma unroll
-                    for (int d = 0; d < DB_OWN; ++d) probe = product_of<T>(values_at(tile, kb, step, d), u32x4{0u, 0u, 0u, 0u}, probe);
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum += probe[e];
-            bool strange = __any(sum != 0.f) != 0;
-            if constexpr (FS > 1) strange = __syncthreads_or(strange) != 0;     // (the wavefronts of a row go the same way)
-            if (__builtin_expect(strange, 0)) return strange_tile(tile, key0, places);
-        }
         f32x16 s[KB];
         unsigned sees[KB];
 #pragma unroll
@@ -527,6 +509,38 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
 #pragma unroll
             for (int i = 0; i < KC_OWN; ++i)
                 s[kb] = product_of<T>(piece_at(tile + kb * 32 * ROWB + k_row + fs * KC_OWN * 32 + (k_piece ^ (i * 32))), q[i], s[kb]);
+        }
+        if constexpr (MASKED) {
+            // Whether any value is no finite number: their products with zeros are zeros unless it is.  (bfloat16 by the matrix cores, beside the scores' products,
+            // which wait for other results; float32's are eight times as long as the few vector instructions.)
+            float sum = 0.f;
+            if constexpr (SZ == 2) {
+                f32x16 probe;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) probe[e] = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int step = 0; step < STEPS; ++step)
+#pragma unroll
+                        for (int d = 0; d < DB_OWN; ++d) probe = product_of<T>(values_at(tile, kb, step, d), u32x4{0u, 0u, 0u, 0u}, probe);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += probe[e];
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int step = 0; step < STEPS; ++step)
+#pragma unroll
+                        for (int d = 0; d < DB_OWN; ++d) {
+                            const u32x4 v = values_at(tile, kb, step, d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sum = fmaf(__uint_as_float(v[e]), 0.f, sum);
+                        }
+            }
+            bool strange = __any(sum != 0.f) != 0;
+            if constexpr (FS > 1) strange = __syncthreads_or(strange) != 0;     // (the wavefronts of a row go the same way)
+            if (__builtin_expect(strange, 0)) return strange_tile(tile, key0, places);
         }
         if constexpr (FS > 1) {                          // the scores of the other features, from the wavefronts that have them
             tree_f32x4* const given = reinterpret_cast<tree_f32x4*>(smem + NS * KS * TILE) + lane;
