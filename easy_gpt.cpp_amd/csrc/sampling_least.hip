@@ -39,11 +39,11 @@ __device__ __forceinline__ void load_part(const float* __restrict__ row, int bef
     }
 }
 
-// What a row is cut by.  Its list holds the tokens of a weight of at least `floor`, by a bound on the logit, max + reach, that stands a thousandth lower (the
-// weight's argument, below 2^7, is rounded twice), and of the k largest.  top-p behind top-k refers to the mass of all k.  A short row is listed
+// What a row is cut by.  Its list holds the tokens of a weight of at least `floor`, by a bound on the logit, max + reach, and of the k largest; either bound
+// stands a thousandth of the temperature lower (a weight's argument, below 2^7, is rounded twice, and equal weights are kept together).  top-p behind top-k refers to the mass of all k.  A short row is listed
 // whole, a greedy one's maxima, and those of a row that nothing of it bounds.
 struct RowCuts {
-    float p, u, least, floor, inv_t, reach;
+    float p, u, least, floor, inv_t, reach, slack;
     int k;
     bool greedy, by_count, by_mass, count_bounds, lists, sums_mass;
 };
@@ -64,6 +64,7 @@ __device__ __forceinline__ RowCuts cuts_of(int r, const float* __restrict__ temp
     c.count_bounds = !c.greedy && !whole && c.by_count && c.k <= kSampleThreads;
     c.lists = !c.greedy && (whole || c.count_bounds || c.floor > 0.f);
     c.reach = !c.lists ? 0.f : whole || c.floor == 0.f ? -INFINITY : (logf(c.floor) - 1e-3f) * t;
+    c.slack = 1e-3f * t;
     c.sums_mass = c.lists && c.by_mass && !c.by_count;
     return c;
 }
@@ -261,7 +262,8 @@ __device__ __forceinline__ float bound_by_count(float mine, float most, int k, L
     least = -fold_row(-s.min[threadIdx.x % kWaves], MaxOf());
     const float range = most - least;
     if (!(range < INFINITY)) return -INFINITY;               // (an infinity, or nothing at all)
-    const float per_bin = range * (1.0f / (kBins - 1)), bins = range > 0.f ? (kBins - 1) / range : 0.f;
+    // (a range that has no reciprocal is one bin: all of them are beyond its foot)
+    const float per_bin = range * (1.0f / (kBins - 1)), bins = range > 1e-30f ? (kBins - 1) / range : 0.f;
     if (mine > -INFINITY) atomicAdd(&s.count[0][min(kBins - 1, static_cast<int>((mine - least) * bins))], 1u);
     __syncthreads();
     if (threadIdx.x < kWave) {
@@ -313,7 +315,7 @@ __device__ __forceinline__ PartOfRow list_part(const float4 (&v)[kQuads], int fi
         for (int i = 0; i < kQuads; ++i) sum += (share(v[i].x) + share(v[i].y)) + (share(v[i].z) + share(v[i].w));
         part.mass = static_cast<double>(sum);
     }
-    const float bound = fmaxf(part.k_bound, part.max + c.reach);
+    const float bound = fmaxf(part.k_bound - c.slack, part.max + c.reach);
     if (__any(part.mine >= bound)) {                         // a wavefront's tokens take places together
         unsigned long long in[4 * kQuads];
         int found = 0;
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_joined_kernel(
     }
     double mass = 0.0;
     if (c.sums_mass) mass = sum_of_all(t <= last ? mine.mass * static_cast<double>(times_two_to((mine.max - mx) * (c.inv_t * kLog2e))) : 0.0, s);
-    const float bound = fmaxf(k_bound, mx + c.reach);
+    const float bound = fmaxf(k_bound - c.slack, mx + c.reach);
     for (int i = 0; wave + kWaves * i <= last; ++i) {
         const int n = __builtin_amdgcn_readlane(n_of_wave, i);
         if (n > kListedOfPiece) {                            // the piece had more than its list holds, and so has the row

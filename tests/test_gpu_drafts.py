@@ -410,6 +410,23 @@ def test_min_p_with_infinities_and_rows_of_nothing_but_nan(vocab):
         assert got[0] == 7 and got[1] == 0 and got[2] % 2 == 1 and not (5 <= got[3] < 50), (cuts, got)
 
 
+@pytest.mark.parametrize("vocab", [1500, 3000, 40000])
+def test_min_p_among_logits_that_hardly_differ(vocab):
+    # differences below what an exponential or a reciprocal tells from nothing: all weigh the same, every cut leaves all of them
+    g = torch.Generator().manual_seed(12)
+    x = torch.randint(0, 9, (4, vocab), generator=g).float() * 1e-39
+    x[1] *= 1e30                                             # (and one whose differences are no smaller than that: 1e-9)
+    x[2] = 1e6 + torch.randint(0, 2, (vocab,), generator=g).float() * 0.0625
+    u = torch.tensor([0.3, 0.3, 0.0, 0.77])
+    for cuts in ((20, 0.9, 0.5), (20, 1.0, 0.0), (1000, 0.5, 0.1)):
+        got = sample(x, 1.0, *cuts[:2], u, cuts[2])
+        assert got[0] == int(float(u[0]) * vocab) and got[3] == int(float(u[3]) * vocab), (cuts, got)      # (of the uniform numbers in 32 bits)
+        top = torch.nonzero(x[2] == x[2].max()).flatten().tolist()
+        if cuts[0] <= len(top):
+            assert got[2] == top[0], (cuts, got)
+        assert got[1] == int(float(u[1]) * vocab), (cuts, got)   # (weights of 1 and 1 - 1e-9 are the same in 32 bits)
+
+
 def test_rows_of_any_number_of_pieces_agree(monkeypatch):
     # rows that begin between 16 bytes, pieces of a few tokens and of as many as they may have: the tokens are the same
     g = torch.Generator().manual_seed(9)
