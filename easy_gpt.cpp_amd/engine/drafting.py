@@ -21,18 +21,31 @@ class PromptLookup:
             raise ValueError("longest and branches must be greater than 0")
         self.longest, self.branches = longest, branches
         self.tokens: list[int] = []
-        self._places: dict[tuple, list[int]] = {}        # a run -> the indexes behind its latest places, oldest first
+        # by a run's length: the run -> the indexes behind its latest places, oldest first (one place is a number by itself: most
+        # runs have no more, and a prompt's tokens are many: 32,000 take 25 ms so, 120 with a list for each)
+        self._places: list[dict] = [{} for _ in range(longest)]
 
     def extend(self, tokens) -> None:
         """The request goes on with these tokens."""
-        for t in tokens:
-            self.tokens.append(int(t))
-            end = len(self.tokens)
-            for n in range(1, min(self.longest, end) + 1):
-                places = self._places.setdefault(tuple(self.tokens[end - n :]), [])
-                places.append(end)
-                if len(places) > self.branches + 1:      # (the last one is the end itself, behind which nothing is known)
-                    del places[0]
+        known, first = self.tokens, len(self.tokens)
+        known.extend(int(t) for t in tokens)
+        keep = -(self.branches + 1)                      # (the last one is the end itself, behind which nothing is known)
+        for n, places in enumerate(self._places, 1):
+            runs = known[max(first - n + 1, 0) :]
+            for end, run in enumerate(runs if n == 1 else zip(*(runs[i:] for i in range(n))), max(first + 1, n)):
+                before = places.get(run)
+                if before is None:
+                    places[run] = end
+                elif type(before) is int:
+                    places[run] = (before, end)[keep:]
+                else:
+                    places[run] = (*before, end)[keep:]
+
+    def _behind(self, n: int) -> list[int]:
+        """The indexes behind the latest places of the last n tokens, oldest first, their own place aside."""
+        end = len(self.tokens)
+        places = self._places[n - 1].get(self.tokens[-1] if n == 1 else tuple(self.tokens[end - n :]), ())
+        return [p for p in ((places,) if type(places) is int else places) if p < end]
 
     def propose(self, max_nodes: int, max_depth: int) -> tuple[list[int], list[int]]:
         """(tokens, parents) of a tree of at most max_nodes nodes, none deeper than max_depth: node 0 is the request's last
@@ -44,7 +57,7 @@ class PromptLookup:
         tokens, parents = [self.tokens[-1]], [-1]
         children: dict[tuple[int, int], int] = {}
         for n in range(min(self.longest, end), 0, -1):
-            places = [p for p in self._places.get(tuple(self.tokens[end - n :]), ()) if p < end]
+            places = self._behind(n)
             for p in reversed(places):                   # the latest first
                 node = 0
                 for t in self.tokens[p : p + max_depth]:
