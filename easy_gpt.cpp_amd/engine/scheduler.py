@@ -464,6 +464,7 @@ class Scheduler:
             self.engine.finish(r.request_id)
             self.running.remove(r)
             r.status, r.finish_reason, r.t_finish = "finished", reason, time.perf_counter()
+            r.lookup = None
             self.stats.finished += 1
             self.done.append(r)
             finished.append(r)
