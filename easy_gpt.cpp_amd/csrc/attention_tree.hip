@@ -670,6 +670,8 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         if ((window_of + 1) * AHEAD < rounds) next = places_from(from + (window_of + 1) * kWave * kGroup);
         return gone_here();
     };
+    // (a wavefront behind the last row loads its share of the tiles and leaves the pipes to the others; where wavefronts share features all of them meet in a tile)
+    const bool has_rows = FS > 1 || row0 + rb * 32 < rows;
     constexpr int ROUND = KT * KS;
     const int open_end = (min(before, to) - from) / ROUND;
     int round = first_round, stop = min(rounds, max(first_round, (all_see - from + ROUND - 1) / ROUND));
@@ -678,13 +680,13 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         for (; round < stop; ++round) {
             begin_round(round);
             const int tile = round * KS + ksi;
-            if (tile < n_tiles) tile_of(std::true_type{}, tile_at(round), from + tile * KT, here);
+            if (tile < n_tiles && has_rows) tile_of(std::true_type{}, tile_at(round), from + tile * KT, here);
             end_round(round);
         }
         if (round >= rounds) break;
         for (; round < open_end && !gone; ++round) {
             begin_round(round);
-            tile_of(std::false_type{}, tile_at(round), from + (round * KS + ksi) * KT, here);
+            if (has_rows) tile_of(std::false_type{}, tile_at(round), from + (round * KS + ksi) * KT, here);
             gone = end_round(round);
         }
         stop = rounds;
