@@ -22,6 +22,7 @@ namespace egpt {
 
 constexpr int kMaxTreeHead = 256;
 constexpr float kSlack = 8.0f;                   // how far, in powers of two, a row's maximum may run ahead of the one in use
+constexpr float kFar = 4096.0f;                  // how large a maximum, as a power of two, may be for its product with the scale to be rounded
 constexpr int kMostParts = 64;                   // of a request's keys: a lane each where they are joined
 
 // One row's view of the keys: the tokens before the tree from `lo` on, and the nodes of its bits.
@@ -440,6 +441,7 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
+    bool far = false;                                            // some row's maximum lies beyond kFar
     const float scale2 = fabsf(z.scale) * 1.4426950408889634f;   // exponentials are taken to the base 2
     const int my_key = SZ == 2 ? (lr & 3) | (lr >> 1 & 4) | (lr << 1 & 8) | (lr & 16) : lr;
     const int k_row = my_key * ROWB, k_piece = (lh ^ swap_at(lr)) * 16;
@@ -485,6 +487,7 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
             const float m_new = sees ? fmaxf(m_run, dot) : m_run, m_use = m_new == -INFINITY ? 0.f : m_new;
             const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_use) * scale2), w = __builtin_amdgcn_exp2f((dot - m_use) * scale2);
             m_run = m_new;
+            far = far || __any(fabsf(m_run) * scale2 > kFar && m_run != -INFINITY);
             l_run = l_run * alpha + (sees && lh == 0 ? w : 0.f);             // (the halves' sums are added up in the end)
             const char* const values = tile + HALF + key / kGroup * HD * kGroup * SZ;
 #pragma unroll
@@ -605,20 +608,31 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
             const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale2);
             l_run *= alpha;
             m_run = m_new;
+            far = __any(fabsf(m_run) * scale2 > kFar && m_run != -INFINITY) != 0;
 #pragma unroll
             for (int d = 0; d < DB_OWN; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
         }
         const float m_use = m_run == -INFINITY ? 0.f : m_run;
-        [[maybe_unused]] const float m_scaled = m_use * scale2;
+        [[maybe_unused]] float m_scaled = m_use * scale2;
+        if constexpr (SZ == 2) {
+            if (__builtin_expect(far, 0)) {
+                m_scaled = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[kb][e] -= m_use;
+            }
+        }
         u32x4 weights[KB][STEPS];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                // (bfloat16: the argument by one operation, whose error, 2^-24 of the maximum, is nothing beside the probabilities' rounding)
+                // (bfloat16: the argument by one operation; what the rounding of the maximum's product leaves in it, 2^-13 at kFar, is nothing beside the
+                // probabilities' rounding.  Beyond, where it would be, and at 2^31 exceed every exponent, the maximum is taken off first, as float32 has it.)
                 float p = SZ == 2 ? __builtin_amdgcn_exp2f(fmaf(s[kb][e], scale2, -m_scaled)) : __builtin_amdgcn_exp2f((s[kb][e] - m_use) * scale2);
                 if constexpr (MASKED) p = __uint_as_float(__float_as_uint(p) & bit_filled(sees[kb], e / R * 2 * R + e % R));
                 s[kb][e] = p;

@@ -158,6 +158,25 @@ def test_large_and_negative_scales(dtype, hd):
         check_tree(c)
 
 
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (BF16, 256), (F32, 64), (BF16, 20)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_so_large_that_one_key_has_all_the_weight(sign, dtype, hd):
+    # Scores of up to 2^39 times the scale, all exact in 24 bits: products of powers of two and an integer up to 15.  Equal ones are equal, others lie 2^28 hd scale
+    # and more below, where a weight is zero: the greatest ones' values in equal shares, whose rounding and sums alone count.
+    c, _ = plain.tree_case(random.Random(hd), [9, 33], [500, 3000], 4, 2, hd, 16, dtype, DEV)
+    g = torch.Generator().manual_seed(hd)
+    steps = torch.randint(0, 16, c["k_cache"].shape[:3], generator=g).to(DEV)
+    c["k_cache"][:] = (steps * 2.0 ** 14)[..., None].to(dtype)
+    signs = torch.randint(0, 2, (42, 4, 1), generator=g).to(DEV) * 2 - 1
+    c["qkv"][:, : 4 * hd] = (signs * 2.0 ** 14).expand(42, 4, hd).reshape(42, 4 * hd).to(dtype)
+    c["scale"] *= sign
+    want, spread = expected(c)
+    share = 2.0 ** -20 + 2 * 3033 * 2.0 ** -24 + (2.0 ** -8 if dtype == BF16 else 0.0)
+    tol = share * spread + torch.finfo(dtype).eps / 2 * want.abs() * (1 + share) + 1e-30
+    err = (run_tree(c).cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
 @pytest.mark.parametrize("dtype,hd", [(BF16, 64), (F32, 64), (BF16, 20)])
 def test_rows_of_no_request_stay_and_requests_may_be_empty(dtype, hd):
     c, _ = plain.tree_case(random.Random(12), [4, 0, 17, 0], [33, 20, 64, 0], 4, 2, hd, 16, dtype, DEV, parents=None, extra_rows=9)
