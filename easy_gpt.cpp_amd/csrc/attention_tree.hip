@@ -391,7 +391,7 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
     // this lane's row
     const int r = row0 + rb * 32 + lr;
     const int node_at = divided(r, group, z.magic_group);
-    const bool valid = r < rows && qs >= 0 && qs + node_at < z.n_tokens;
+    const bool valid = r < rows && qs >= 0 && node_at < z.n_tokens - qs;
     const int node = valid ? node_at : 0, head = kvh * group + (valid ? r - node * group : 0);
     const int token = qs + node;
     // the first round: with a window the one that has the first key that any row of the workgroup sees
@@ -791,10 +791,10 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __rest
     __shared__ float s_weight[4 * ROWS][kMostParts];
     const int lane = threadIdx.x % kWave, sub = lane % L, in = threadIdx.x / L, b = blockIdx.y;
     const int w = blockIdx.x * 4 * ROWS + in, node = divided(w, nq, magic_heads), head = w - node * nq;
-    const int n = q_len[b], kv = kv_len[b], token = q_start[b] + node;
+    const int n = q_len[b], kv = kv_len[b], qs = q_start[b], token = qs + node;
     const int per = *per_of, parts = min(upper_quotient(rounds_of_keys(kv, round_keys), per, __builtin_amdgcn_rcpf(static_cast<float>(per))), kMostParts);
     if (parts < 2) return;
-    const bool there = node < n && node < nodes && token >= 0 && token < n_tokens;
+    const bool there = node < n && node < nodes && qs >= 0 && node < n_tokens - qs;
     if (!__any(there)) return;
     const size_t row = there ? static_cast<size_t>(token) * nq + head : 0, step = static_cast<size_t>(n_tokens) * nq;
     const int quads = hd / 4, at = min(sub, quads - 1) * 4;

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(64) void accept_drafts_kernel(const int32_t* __rest
                                                            int32_t* __restrict__ count, int32_t* __restrict__ accepted) {
     const int b = blockIdx.x, lane = threadIdx.x;
     const int at = q_start[b], n = min(q_len[b], kTreeNodes);
-    const bool here = lane < n && at >= 0 && at + lane < n_tokens;
+    const bool here = lane < n && at >= 0 && lane < n_tokens - at;
     const int token = here ? tokens[at + lane] : -1, parent = here ? parents[at + lane] : -1, next = here ? sampled[at + lane] : -1;
     int length = 0, mine = -1;
     if (n > 0) {
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void keep_drafts_kernel(const int32_t* __restr
         const int n = min(min(count[b], path_width), kTreeNodes), before = start[b];
         const int node = lane < n ? path[static_cast<size_t>(b) * path_width + lane] : -1;
         // (what lies where it belongs stays; what has no page, or would be written over, is not touched)
-        bool moves = node > lane && node < kTreeNodes && before >= 0;
+        bool moves = node > lane && node < kTreeNodes && before >= 0 && before < 0x7fffffff - kTreeNodes;
         int from = -1, to = -1;
         const int of = before + node, into = before + lane;
         if (moves && of / page_size < table_width) {

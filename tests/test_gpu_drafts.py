@@ -599,6 +599,27 @@ def test_keep_touches_nothing_it_cannot_place():
     assert torch.equal(k, k0) and torch.equal(v, v0)
 
 
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 31 - 5, -(2 ** 31), -1])
+def test_starts_far_from_everything_are_nobody_s(far):
+    # (a start to which a node's number cannot be added in 32 bits)
+    k, v = torch.randn((2, 6, 1, 16, 8), device=DEV), torch.randn((2, 6, 1, 8, 16), device=DEV)
+    k0, v0 = k.clone(), v.clone()
+    kernels.backend().keep_drafts(k, v, i32([[2, 3], [4, 5]]), i32([far, far]), i32([[0, 20, 21], [0, 18, 22]]), i32([3, 3]))
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    path, count, accepted = kernels.backend().accept_drafts(i32([1, 2, 3]), i32([-1, 0, 1]), i32([2, 3, 9]), i32([far, 0]), i32([40, 3]))
+    assert accepted[1].tolist()[:4] == [2, 3, 9, -1] and count[1] == 3 and path[1].tolist()[:4] == [0, 1, 2, -1]
+    assert bool((accepted[0] == -1).all())
+    for hd, dtype in ((64, BF16), (20, F32)):
+        c, _ = plain.tree_case(random.Random(31), [6, 9], [40, 900], 4, 2, hd, 16, dtype, DEV)
+        whole = run_tree(c)
+        c["q_start"][0 if far < 0 else 1] = far                  # (starts ascend)
+        got = run_tree(c)
+        there = slice(6, 15) if far < 0 else slice(0, 6)
+        nobody = slice(0, 6) if far < 0 else slice(6, 15)
+        assert torch.equal(got[there], whole[there]), (hd, dtype)
+        assert far < 0 or bool(got[nobody].isnan().all())
+
+
 def test_walk_and_move_refusals():
     k = kernels.backend()
     tok, par, sam, qs, ql = walk_case(random.Random(1), [5, 3])
