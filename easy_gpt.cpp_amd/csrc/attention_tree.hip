@@ -192,6 +192,9 @@ struct TreeSizes {
     float scale;
 };
 
+// What a difference of scores is an exponent of 2 by.  (A negative scale turns the queries' signs.)
+__host__ __device__ __forceinline__ float base_2_scale(float scale) { return fabsf(scale) * 1.4426950408889634f; }
+
 template <typename T, int HD, int RB, int KS, int KT, int NS, int FS>
 constexpr int tree_lds() {
     constexpr int stages = NS * KS * 2 * KT * HD * static_cast<int>(sizeof(T)), join = KS * RB * 64 * (HD / 2 + 2) * 4;
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
     bool far = false;                                            // some row's maximum lies beyond kFar
-    const float scale2 = fabsf(z.scale) * 1.4426950408889634f;   // exponentials are taken to the base 2
+    const float scale2 = base_2_scale(z.scale);
     const int my_key = SZ == 2 ? (lr & 3) | (lr >> 1 & 4) | (lr << 1 & 8) | (lr & 16) : lr;
     const int k_row = my_key * ROWB, k_piece = (lh ^ swap_at(lr)) * 16;
     const int v_row = lr * kGroup * SZ + (SZ == 2 ? (lh ^ (lr >> 3 & 1)) * 16 : ((lh ^ (lr >> 2 & 3)) * 16));
@@ -774,19 +777,19 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
             }
     }
     if (!whole && lh == 0 && ksi == 0 && fs == 0) {
-        part_ml[mine * 2] = m_all * scale2;
+        part_ml[mine * 2] = m_all;                       // (as it is: its product with the scale would be rounded, and may be no number)
         part_ml[mine * 2 + 1] = l;
     }
 }
 
-// The parts of a request's keys joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  A row has L lanes, four features each, and a wavefront 64 / L rows; the
+// The parts of a request's keys joined, with s = scale log2 e: out = sum_p 2^(s (m_p - M)) o_p / sum_p 2^(s (m_p - M)) l_p.  A row has L lanes, four features each, and a wavefront 64 / L rows; the
 // lanes take the parts' maxima and sums between them, so that the weights of all are known after one trip, and then the parts' sums, kAhead on their way at a time.  A
 // part that saw nothing weighs nothing, whatever it holds.  (64 uneven requests at heads of 64: a row to a
 // wavefront 8.8 us, four 5.6.)
 template <typename T, int L>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __restrict__ q_len, const int32_t* __restrict__ kv_len, const int32_t* __restrict__ q_start,
                                                            const float* __restrict__ part_ml, const float* __restrict__ part_o, const int* __restrict__ per_of, int round_keys,
-                                                           int nq, unsigned magic_heads, int nodes, int n_tokens, int hd, T* __restrict__ out) {
+                                                           int nq, unsigned magic_heads, int nodes, int n_tokens, int hd, float scale2, T* __restrict__ out) {
     constexpr int kAhead = 8, ROWS = kWave / L, OWN = kMostParts / L;
     __shared__ float s_weight[4 * ROWS][kMostParts];
     const int lane = threadIdx.x % kWave, sub = lane % L, in = threadIdx.x / L, b = blockIdx.y;
@@ -822,7 +825,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const int32_t* __rest
 #pragma unroll
     for (int j = 0; j < OWN; ++j) {
         if (j > 0 && j * L >= parts) continue;
-        const float weight = l[j] != 0.f ? __builtin_amdgcn_exp2f(m[j] - most) : 0.f;
+        const float weight = l[j] != 0.f ? __builtin_amdgcn_exp2f((m[j] - most) * scale2) : 0.f;
         total = fmaf(weight, l[j], total);
         s_weight[in][sub + j * L] = l[j] != 0.f ? weight : -1.f;      // (of a part that saw nothing, whose sums may be anything)
     }
@@ -882,7 +885,8 @@ static int launch_tree(const void* qkv, void* out, float* part_o, float* part_ml
     if (parts > 1) {
         constexpr int L = HD <= 64 ? 16 : HD <= 128 ? 32 : 64, rows_of_group = 4 * (kWave / L);
         tree_combine_kernel<T, L><<<dim3((max_q_len * z.nq + rows_of_group - 1) / rows_of_group, n_seqs), 256, 0, s>>>(
-            q_len, kv_len, q_start, part_ml, part_o, per, KT * KS, z.nq, magic_of(z.nq), max_q_len, z.n_tokens, z.hd, static_cast<T*>(out));
+            q_len, kv_len, q_start, part_ml, part_o, per, KT * KS, z.nq, magic_of(z.nq), max_q_len, z.n_tokens, z.hd, base_2_scale(z.scale),
+            static_cast<T*>(out));
         EGPT_CHECK_LAUNCH();
     }
     return EGPT_OK;

@@ -1,0 +1,90 @@
+"""Attention for trees of drafted tokens in every shape of the matrix-core kernel, with the keys of a request in one part and in several, against
+64-bit arithmetic."""
+import math
+import random
+
+import pytest
+import torch
+
+import plain_drafts as plain
+from easy_gpt.cpp_amd import kernels
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+# (type, head size) and the shapes that the kernel has for it: 10 * (blocks of 32 rows to a workgroup) + wavefronts that share a block's keys
+SHAPES = [(BF16, 64, 14), (BF16, 64, 22), (BF16, 64, 41), (BF16, 128, 14), (BF16, 128, 22), (BF16, 128, 81), (BF16, 256, 11), (BF16, 256, 21),
+          (BF16, 256, 41), (F32, 64, 14), (F32, 64, 22), (F32, 128, 22), (F32, 128, 41), (F32, 256, 21)]
+every_shape = pytest.mark.parametrize("dtype,hd,shape", SHAPES, ids=lambda v: str(v).replace("torch.", ""))
+in_parts = pytest.mark.parametrize("parts", [1, 5])
+
+
+def run_shape(monkeypatch, c, shape, parts, out=None):
+    """The call, with this shape and at most so many parts of a request's keys, all of them used."""
+    k = kernels.backend()
+    if out is None:
+        out = torch.full((c["qkv"].shape[0], c["nq"] * c["hd"]), math.nan, dtype=c["qkv"].dtype, device=DEV)
+    lens, rows = c["q_len"].tolist(), 32 * (shape // 10)
+    blocks = sum(-(-n * (c["nq"] // c["nkv"]) // rows) for n in lens) * c["nkv"]
+    asked = []
+    with monkeypatch.context() as m:
+        m.setattr(k, "_tree_shape", lambda *a: asked.append(a) or (shape, parts, blocks * parts), raising=False)
+        k.tree_attention(c["qkv"], out, c["k_cache"], c["v_cache"], c["block_table"], c["q_start"], c["q_len"], c["kv_len"], c["visible"], c["nq"], c["nkv"],
+                         c["hd"], c["page_size"], c["scale"], max(lens), max(c["kv_len"].tolist()), window=c["window"], positions=c["positions"])
+    assert asked                                             # (the kernel that has shapes)
+    return out
+
+
+def expected(c):
+    names = ("qkv", "k_cache", "v_cache", "block_table", "q_start", "q_len", "kv_len", "visible", "nq", "nkv", "hd", "page_size", "scale",
+             "window", "positions")
+    return plain.tree_attention(*(c[n] for n in names))
+
+
+def exact_scores_tolerance(c, spread, want):
+    """Where scores are exact, what is left is an exponential (2^-21, its argument's rounding included), sums over the L weights, the rounding of bfloat16's
+    weights to 2^-8 and that of the result."""
+    bf16 = c["qkv"].dtype == BF16
+    share = 2.0 ** -20 + 2 * int(c["kv_len"].max()) * 2.0 ** -24 + (2.0 ** -8 if bf16 else 0.0)
+    return share * spread + torch.finfo(c["qkv"].dtype).eps / 2 * want.abs() * (1 + share) + 1e-30
+
+
+def within(got, want, tol):
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@in_parts
+@every_shape
+def test_large_scores_that_differ_by_little(monkeypatch, dtype, hd, shape, parts, sign):
+    # Scores 2^20 - d, exact in 24 bits, d from 0 to 3 and the same for some 180 keys: parts have maxima that differ by 1 to 3.
+    c, _ = plain.tree_case(random.Random(hd), [9, 6], [700, 1500], 4, 2, hd, 16, dtype, DEV)
+    c["scale"] = float(sign)
+    c["qkv"].zero_()
+    c["qkv"].view(15, 8, hd)[:, :4, 0] = sign * 1024.0
+    c["qkv"].view(15, 8, hd)[:, :4, 1] = sign * 1.0
+    pages = c["block_table"].cpu()
+    c["k_cache"].zero_()
+    for b, kv in enumerate(c["kv_len"].tolist()):
+        for j in range(kv):
+            c["k_cache"][int(pages[b, j // 16]), :, j % 16, 0] = 1024.0
+            c["k_cache"][int(pages[b, j // 16]), :, j % 16, 1] = -float((3, 1, 0, 2)[j // 181 % 4])
+            c["v_cache"][int(pages[b, j // 16]), :, :, j % 16] = (-1.0) ** (j // 181)       # (a weight that is off is off in the result)
+    want, spread = expected(c)
+    within(run_shape(monkeypatch, c, shape, parts), want, exact_scores_tolerance(c, spread, want))
+
+
+@in_parts
+@every_shape
+def test_scores_beyond_32_bits_once_scaled(monkeypatch, dtype, hd, shape, parts):
+    # Products of 2^126 and 0, a scale of 8: the keys that have the greatest share the weight.
+    c, _ = plain.tree_case(random.Random(hd + 1), [5, 7], [700, 1100], 4, 2, hd, 16, dtype, DEV)
+    c["scale"] = 8.0
+    c["qkv"].zero_()
+    c["qkv"].view(12, 8, hd)[:, :4, 0] = 2.0 ** 63
+    g = torch.Generator().manual_seed(hd)
+    c["k_cache"].zero_()
+    c["k_cache"][..., 0] = (torch.randint(0, 2, c["k_cache"].shape[:3], generator=g) * 2.0 ** 63).to(dtype).to(DEV)
+    want, spread = expected(c)
+    within(run_shape(monkeypatch, c, shape, parts), want, exact_scores_tolerance(c, spread, want))
