@@ -680,21 +680,20 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         const int key = from + (window_of * kWave + lane) * kGroup;
         return __any(here.page < 0 && key < before && key + kGroup > all_see) != 0;
     };
+    bool gone = gone_here();                                     // some key of `here` that all rows would see is in no page
     auto end_round = [&](int round) {
-        if ((round + 1) % AHEAD != 0) return false;
+        if ((round + 1) % AHEAD != 0) return;
         here = next;
         ++window_of;
         if ((window_of + 1) * AHEAD < rounds) next = places_from(from + (window_of + 1) * kWave * kGroup);
-        return gone_here();
+        gone = gone_here();
     };
     // (a wavefront behind the last row loads its share of the tiles and leaves the pipes to the others; where wavefronts share features all of them meet in a tile)
     const bool has_rows = FS > 1 || row0 + rb * 32 < rows;
     constexpr int ROUND = KT * KS;
-    const int open_end = (min(before, to) - from) / ROUND;
-    int round = first_round, stop = min(rounds, max(first_round, (all_see - from + ROUND - 1) / ROUND));
-    bool gone = gone_here();
-    for (;;) {
-        for (; round < stop; ++round) {
+    const int open_from = (all_see - from + ROUND - 1) / ROUND, open_end = (min(before, to) - from) / ROUND;
+    for (int round = first_round;;) {
+        for (; round < rounds && (gone || round < open_from || round >= open_end); ++round) {
             begin_round(round);
             const int tile = round * KS + ksi;
             if (tile < n_tiles && has_rows) tile_of(std::true_type{}, tile_at(round), from + tile * KT, here);
@@ -704,9 +703,8 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         for (; round < open_end && !gone; ++round) {
             begin_round(round);
             if (has_rows) tile_of(std::false_type{}, tile_at(round), from + (round * KS + ksi) * KT, here);
-            gone = end_round(round);
+            end_round(round);
         }
-        stop = rounds;
     }
     float l = fold_32_apart(l_run, AddOf());
 

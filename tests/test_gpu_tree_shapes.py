@@ -88,3 +88,19 @@ def test_scores_beyond_32_bits_once_scaled(monkeypatch, dtype, hd, shape, parts)
     c["k_cache"][..., 0] = (torch.randint(0, 2, c["k_cache"].shape[:3], generator=g) * 2.0 ** 63).to(dtype).to(DEV)
     want, spread = expected(c)
     within(run_shape(monkeypatch, c, shape, parts), want, exact_scores_tolerance(c, spread, want))
+
+
+@in_parts
+@every_shape
+def test_missing_pages_behind_the_last_masked_round_of_a_window(monkeypatch, dtype, hd, shape, parts):
+    # The rows' windows begin at keys 1,001 to 1,008, in the last round before key 1,024, where the next 64 groups of 16 keys begin; some of those are in no page.
+    c, _ = plain.tree_case(random.Random(hd + 2), [8, 8], [3000, 2100], 4, 2, hd, 16, dtype, DEV, window=2000, parents=[list(range(-1, 7))] * 2)
+    c["positions"][8:] += 900                                # (the second request's begin there as well)
+    c["v_cache"] += 3.0                                      # (values of one sign: weights for keys that are not there show)
+    c["block_table"][:, [70, 95]] = -1
+    clean = dict(c, block_table=c["block_table"].clone())
+    c["block_table"][0, 100] = c["k_cache"].shape[0] + 3     # a page that the cache does not have is none either
+    clean["block_table"][0, 100] = -1
+    want, spread = expected(clean)
+    got = run_shape(monkeypatch, c, shape, parts)
+    within(got, want, plain.tree_tolerance(clean, spread, want))
