@@ -316,7 +316,8 @@ __device__ __forceinline__ PartOfRow list_part(const float4 (&v)[kQuads], int fi
         part.mass = static_cast<double>(sum);
     }
     const float bound = fmaxf(part.k_bound - c.slack, part.max + c.reach);
-    if (__any(part.mine >= bound)) {                         // a wavefront's tokens take places together
+    // (a part of nothing but -infinity and NaN has no bound, and no candidates either)
+    if (__any(part.mine >= bound && part.max > -INFINITY)) {     // a wavefront's tokens take places together
         unsigned long long in[4 * kQuads];
         int found = 0;
 #pragma unroll
@@ -497,7 +498,9 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_joined_kernel(
     // What may be asked for at once is: a piece to a thread, and of its wavefront's two first pieces an entry to a lane (where the piece listed so many).
     const int last = pieces - 1, shares = shares_of_piece(pieces);
     const PieceOfRow mine = found[at + min(t, last)];
-    const int of_wave = wave + kWaves * lane, n_of_wave = of_wave <= last ? found[at + of_wave].listed : 0;
+    const int of_wave = wave + kWaves * lane;
+    int n_of_wave = of_wave <= last ? found[at + of_wave].listed : 0;
+    const float max_of_wave = of_wave <= last ? found[at + of_wave].max : -INFINITY;
     uint2 early[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) early[i] = lists[(at + min(wave + kWaves * i, last)) * kListedOfPiece + lane];
@@ -512,9 +515,12 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_joined_kernel(
     double mass = 0.0;
     if (c.sums_mass) mass = sum_of_all(t <= last ? mine.mass * static_cast<double>(times_two_to((mine.max - mx) * (c.inv_t * kLog2e))) : 0.0, s);
     const float bound = fmaxf(k_bound - c.slack, mx + c.reach);
+    // (a piece far below the row's maximum, masked by a large negative number or flat, listed by a bound of its own: nothing of it reaches the row's.
+    // 64 rows of 151,936 with top-k, top-p and min-p, five sixths at -10^9: 20.1 us, 291 where such a piece's list counted; with min-p alone 14.2, 43.7)
+    if (max_of_wave < bound) n_of_wave = 0;
     for (int i = 0; wave + kWaves * i <= last; ++i) {
         const int n = __builtin_amdgcn_readlane(n_of_wave, i);
-        if (n > kListedOfPiece) {                            // the piece had more than its list holds, and so has the row
+        if (n > kListedOfPiece) {                            // more than its list holds, some of which the row's may need: the row is walked
             if (lane == 0) atomicAdd(&s.listed, kListed + 1);
             continue;
         }
