@@ -56,8 +56,8 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
         if (q_start[mid] <= t) lo = mid; else hi = mid - 1;
         b = lo;
     }
-    const int n = q_len[b], i = t - q_start[b];
-    if (i < 0 || i >= n) return;                             // nobody's row stays as it was
+    const int n = q_len[b], qs = q_start[b], i = t - max(qs, 0);
+    if (qs < 0 || i < 0 || i >= n) return;                   // nobody's row stays as it was
     const int kv = static_cast<int>(min(static_cast<long long>(kv_len[b]), static_cast<long long>(table_width) * page_size));
     const int before = kv_len[b] - n;
     const TreeRow row{window > 0 ? max(0, positions[t] - window + 1) : 0, before, kv, static_cast<unsigned long long>(visible[t])};

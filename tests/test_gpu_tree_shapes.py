@@ -104,3 +104,18 @@ def test_missing_pages_behind_the_last_masked_round_of_a_window(monkeypatch, dty
     want, spread = expected(clean)
     got = run_shape(monkeypatch, c, shape, parts)
     within(got, want, plain.tree_tolerance(clean, spread, want))
+
+
+@pytest.mark.parametrize("far", [-1, -3, -(2 ** 31), 2 ** 31 - 5, 2 ** 31 - 1])
+@pytest.mark.parametrize("hd,dtype", [(64, BF16), (20, BF16), (64, F32), (20, F32)])
+def test_rows_of_a_request_that_begins_nowhere_stay(hd, dtype, far):
+    # (starts ascend)
+    c, _ = plain.tree_case(random.Random(31), [6, 9], [40, 90], 4, 2, hd, 16, dtype, DEV)
+    call = lambda out: kernels.backend().tree_attention(c["qkv"], out, c["k_cache"], c["v_cache"], c["block_table"], c["q_start"], c["q_len"], c["kv_len"],
+                                                        c["visible"], 4, 2, hd, 16, c["scale"], 9, 99) or out
+    whole = call(torch.full((15, 4 * hd), math.nan, dtype=dtype, device=DEV))
+    assert bool(whole.isfinite().all())
+    c["q_start"][0 if far < 0 else 1] = far
+    got = call(torch.full((15, 4 * hd), math.nan, dtype=dtype, device=DEV))
+    there, nobody = (slice(6, 15), slice(0, 6)) if far < 0 else (slice(0, 6), slice(6, 15))
+    assert torch.equal(got[there], whole[there]) and bool(got[nobody].isnan().all())
