@@ -63,7 +63,9 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
     const TreeRow row{window > 0 ? max(0, positions[t] - window + 1) : 0, before, kv, static_cast<unsigned long long>(visible[t])};
     const int kvh = h / (nq / nkv);
     const T* q = qkv + static_cast<size_t>(t) * (nq + 2 * nkv) * hd + h * hd;
-    for (int d = threadIdx.x; d < hd; d += kWave * kTreeWaves) q_s[d] = to_float(q[d]);
+    // (the scale is for differences of products alone, which are exact where large ones are near; a negative one turns the query)
+    const float steep = fabsf(scale);
+    for (int d = threadIdx.x; d < hd; d += kWave * kTreeWaves) q_s[d] = scale < 0.f ? -to_float(q[d]) : to_float(q[d]);
     __syncthreads();
     const int32_t* table = block_table + static_cast<size_t>(b) * table_width;
     const size_t head_size = static_cast<size_t>(page_size) * hd;
@@ -83,12 +85,12 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
             const T* kr = k_cache + (static_cast<size_t>(page) * nkv + kvh) * head_size + static_cast<size_t>(j % page_size) * hd;
             float dot = 0.f;
             for (int d = 0; d < hd; ++d) dot = fmaf(q_s[d], to_float(kr[d]), dot);
-            s = dot * scale;
+            s = dot;
         }
         const float m_new = fmaxf(m_run, wave_max(s));
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float pj = sees ? expf(s - m_use) : 0.f;
-        const float alpha = expf(m_run - m_use);
+        const float pj = sees ? expf((s - m_use) * steep) : 0.f;
+        const float alpha = m_run == -INFINITY ? 0.f : expf((m_run - m_use) * steep);
         l_run = l_run * alpha + wave_sum(pj);
         m_run = m_new;
 #pragma unroll
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) {
         // (a wavefront that saw nothing weighs nothing; one whose scores are infinite or no number makes the row one)
-        share[w] = part_ml[w][1] == 0.f ? 0.f : expf(part_ml[w][0] - m_all);
+        share[w] = part_ml[w][1] == 0.f ? 0.f : expf((part_ml[w][0] - m_all) * steep);
         l_all = fmaf(part_ml[w][1], share[w], l_all);
     }
     T* o = out + static_cast<size_t>(t) * nq * hd + h * hd;

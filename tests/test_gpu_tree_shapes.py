@@ -107,7 +107,7 @@ def test_missing_pages_behind_the_last_masked_round_of_a_window(monkeypatch, dty
 
 
 @pytest.mark.parametrize("far", [-1, -3, -(2 ** 31), 2 ** 31 - 5, 2 ** 31 - 1])
-@pytest.mark.parametrize("hd,dtype", [(64, BF16), (20, BF16), (64, F32), (20, F32)])
+@pytest.mark.parametrize("hd,dtype", [(64, BF16), (20, BF16), (64, F32), (22, F32)])
 def test_rows_of_a_request_that_begins_nowhere_stay(hd, dtype, far):
     # (starts ascend)
     c, _ = plain.tree_case(random.Random(31), [6, 9], [40, 90], 4, 2, hd, 16, dtype, DEV)
@@ -119,3 +119,32 @@ def test_rows_of_a_request_that_begins_nowhere_stay(hd, dtype, far):
     got = call(torch.full((15, 4 * hd), math.nan, dtype=dtype, device=DEV))
     there, nobody = (slice(6, 15), slice(0, 6)) if far < 0 else (slice(0, 6), slice(6, 15))
     assert torch.equal(got[there], whole[there]) and bool(got[nobody].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("scale", [22 ** -0.5, -0.3, 8.0])
+def test_large_scores_of_heads_that_the_matrix_cores_do_not_take(scale, dtype):
+    # Products of 2^20 - d, exact in 24 bits; and of 2^126 and 0, whose scaled scores are beyond 32 bits at the greatest scale.
+    c, _ = plain.tree_case(random.Random(41), [9, 6], [700, 1500], 4, 2, 22, 16, dtype, DEV)
+    c["scale"] = scale
+    c["qkv"].zero_()
+    sign = 1.0 if scale > 0 else -1.0
+    c["qkv"].view(15, 8, 22)[:, :4, 0] = sign * 1024.0
+    c["qkv"].view(15, 8, 22)[:, :4, 1] = sign * 1.0
+    pages = c["block_table"].cpu()
+    c["k_cache"].zero_()
+    for b, kv in enumerate(c["kv_len"].tolist()):
+        for j in range(kv):
+            c["k_cache"][int(pages[b, j // 16]), :, j % 16, 0] = 1024.0
+            c["k_cache"][int(pages[b, j // 16]), :, j % 16, 1] = -float((3, 1, 0, 2)[j // 181 % 4])
+            c["v_cache"][int(pages[b, j // 16]), :, :, j % 16] = (-1.0) ** (j // 181)
+    for far in (False, True):
+        if far:
+            c["qkv"].view(15, 8, 22)[:, :4, 0] = sign * 2.0 ** 63
+            c["qkv"].view(15, 8, 22)[:, :4, 1] = 0.0
+            c["k_cache"][..., 0] = (c["k_cache"][..., 1] == 0).to(dtype) * 2.0 ** 63
+        want, spread = expected(c)
+        out = torch.empty((15, 88), dtype=dtype, device=DEV)
+        kernels.backend().tree_attention(c["qkv"], out, c["k_cache"], c["v_cache"], c["block_table"], c["q_start"], c["q_len"], c["kv_len"], c["visible"], 4, 2,
+                                         22, 16, scale, 9, 1506)
+        within(out, want, exact_scores_tolerance(c, spread, want))
