@@ -409,7 +409,7 @@ int egpt_sample_min_p(const float* logits, const float* temperature, const int32
 // ---- drafted tokens (attention_tree.hip, drafts.hip)
 // Attention for trees: operands as egpt_paged_attention; the last q_len[b] of a request's kv_len[b] tokens are its nodes.  visible int64
 // [n_tokens]: bit m of a node's number says that it reads node m.  window > 0: a node reads the tokens before the tree from place positions[t] -
-// window + 1 on.  n_pages: the caches' pages; a table's entry outside them is read as no page.  Any head size up to 256, any page size.
+// window + 1 on.  n_pages: the caches' pages; a table's entry outside them is read as no page.  Any head size up to 256, any page size, tables of at most 2^30 tokens.
 int egpt_tree_attention_generic(const void* qkv, void* out, const void* k_cache, const void* v_cache, const int32_t* block_table, int table_width,
                                 int n_pages, const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len, const long long* visible,
                                 const int32_t* positions, int n_seqs, int n_tokens, int nq, int nkv, int hd, int page_size, float scale, int window,

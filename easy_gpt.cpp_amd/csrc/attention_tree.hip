@@ -905,7 +905,8 @@ extern "C" int egpt_tree_attention_generic(const void* qkv, void* out, const voi
     if (n_seqs <= 0 || n_tokens < 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || hd <= 0 || page_size <= 0 || table_width <= 0 || window < 0 ||
         n_pages < 0 || dtype < 0 || dtype > 1)
         return EGPT_BAD_ARGUMENT;
-    if (hd > kMaxTreeHead || nq > 65535) return EGPT_UNSUPPORTED_SIZE;
+    // (a key's number and the step to the next ones of a wavefront are added in 32 bits)
+    if (hd > kMaxTreeHead || nq > 65535 || static_cast<long long>(table_width) * page_size > 1LL << 30) return EGPT_UNSUPPORTED_SIZE;
     if (n_tokens == 0) return EGPT_OK;
     auto launch = [&](auto zero) {
         using T = decltype(zero);

@@ -2255,8 +2255,8 @@ class HipKernels(KernelBackend):
             raise ValueError(f"head size {hd} is not supported by the attention kernels (1 to {self.max_head_dim})")
         if not 0 <= max_q_len <= self.max_tree_nodes:
             raise ValueError(f"a request's tree has at most {self.max_tree_nodes} nodes, not {max_q_len}")
-        if window < 0:
-            raise ValueError("the window must be >= 0")
+        if not 0 <= window < 1 << 31:
+            raise ValueError("the window must be >= 0 and below 2^31")
         try:
             t, dtype, device, pages = qkv.shape[0], qkv.dtype, qkv.get_device(), k_cache.shape[0]
             usual = (dtype in _DT and device == torch._C._cuda_getDevice() and qkv.shape == (t, (nq + 2 * nkv) * hd) and qkv.is_contiguous()

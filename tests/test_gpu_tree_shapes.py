@@ -148,3 +148,11 @@ def test_large_scores_of_heads_that_the_matrix_cores_do_not_take(scale, dtype):
         kernels.backend().tree_attention(c["qkv"], out, c["k_cache"], c["v_cache"], c["block_table"], c["q_start"], c["q_len"], c["kv_len"], c["visible"], 4, 2,
                                          22, 16, scale, 9, 1506)
         within(out, want, exact_scores_tolerance(c, spread, want))
+
+
+@pytest.mark.parametrize("window", [-1, 1 << 31, (1 << 32) + 5])
+def test_windows_that_32_bits_do_not_hold_are_refused(window):
+    c, _ = plain.tree_case(random.Random(42), [4], [20], 4, 2, 64, 16, BF16, DEV, window=9)
+    c["window"] = window
+    with pytest.raises(ValueError):
+        run_shape(pytest.MonkeyPatch(), c, 14, 1)
