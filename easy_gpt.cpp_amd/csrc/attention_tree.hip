@@ -17,6 +17,7 @@
 #include "api.h"
 #include "common.h"
 #include "lds_loads.h"
+#include "tree_loads.h"
 
 namespace egpt {
 
@@ -366,8 +367,8 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
     // (16 lanes read 256 bytes, all banks, at a time: their rows' pieces lie in 16 different places, two rows of 128 bytes side by side)
     auto swap_at = [](int lane_row) { return PIECES >= 16 ? lane_row & 15 : lane_row >> 1 & 7; };
     auto swap_of = [&](int key) { return swap_at(SZ == 2 ? (key & 3) | (key >> 1 & 4) | (key << 1 & 8) : key); };      // bfloat16: bits 2 and 3 exchanged
-    const int k_at = lane / PIECES * key_bytes, k_place = lane % PIECES ^ swap_of(lane / PIECES);
-    const int v_at = lane / SZ * z.page_size * SZ + (SZ == 2 ? lane % 2 ^ (lane >> 4 & 1) : (lane % 4) ^ (lane / SZ >> 2 & 3)) * 16;       // (features past the head's lie past the resource's end)
+    const int k_row_of_lane = lane / PIECES, k_place = lane % PIECES ^ swap_of(k_row_of_lane);
+    const int v_at = value_lane(lane, SZ, z.page_size, z.hd, kNowhere);
     const int n_tiles = (groups * kGroup + KT - 1) / KT, rounds = (n_tiles + KS - 1) / KS;
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)smem));
     // (`places`: those of the 64 groups that the round's keys are among)
@@ -378,16 +379,21 @@ __global__ __launch_bounds__(64 * RB * KS * FS, HD * static_cast<int>(sizeof(T))
         for (int o = 0; o < OWN; ++o) {
             const int page = g0 + o < groups ? __builtin_amdgcn_readlane(places.page, (g0 + o) % kWave) : -1;
             const int off = __builtin_amdgcn_readlane(places.off, (g0 + o) % kWave);
+            const bool missing = page < 0;
             const size_t at = static_cast<size_t>(max(page, 0)) * page_bytes;
-            const r_i32x4 keys = buffer_of(k_head + at + static_cast<size_t>(off) * key_bytes, page < 0 ? 0 : kGroup * key_bytes);
-            const r_i32x4 values = buffer_of(v_head + at + static_cast<size_t>(off) * SZ, page < 0 ? 0 : head_bytes - static_cast<size_t>(off) * SZ);
+            const char* const keys = k_head + at + static_cast<size_t>(off) * key_bytes;
+            const char* const values = v_head + at + static_cast<size_t>(off) * SZ;
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
-                const int piece = (k_place ^ swap_of((load_first + j) * KEYS)) * 16;
-                load_1k(keys, piece < key_bytes ? k_at + piece : kNowhere, (load_first + j) * KEYS * key_bytes, base + (o * PER_GROUP + j) * 1024);
+                const GroupLoad from_here = key_load(load_first + j, KEYS, key_bytes, missing);
+                load_1k(buffer_of(keys, from_here.bytes), key_lane(k_row_of_lane, key_bytes, k_place ^ swap_of((load_first + j) * KEYS), kNowhere), from_here.more,
+                        base + (o * PER_GROUP + j) * 1024);
             }
 #pragma unroll
-            for (int j = 0; j < EACH; ++j) load_1k(values, v_at, (load_first + j) * 64 * z.page_size, base + HALF + (o * PER_GROUP + j) * 1024);
+            for (int j = 0; j < EACH; ++j) {
+                const GroupLoad from_here = value_load(load_first + j, SZ, z.page_size, z.hd, static_cast<unsigned>(head_bytes) - off * SZ, missing);
+                load_1k(buffer_of(values, from_here.bytes), v_at, from_here.more, base + HALF + (o * PER_GROUP + j) * 1024);
+            }
         }
     };
     constexpr int AHEAD = kWave * kGroup / (KT * KS);            // rounds that the places of 64 groups serve
