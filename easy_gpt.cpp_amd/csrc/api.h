@@ -391,20 +391,21 @@ int egpt_argmax(const float* logits, int32_t* out, void* scratch, int n_rows, in
 #define EGPT_ARGMAX_STATIC_MAX_ROWS 1024
 int egpt_argmax_static_init(void);
 int egpt_argmax_static(const float* logits, int32_t* out, int n_rows, int vocab, void* stream);
-// weights: scratch for n_rows * vocab floats.
-int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream);
+// weights: scratch for n_rows * vocab floats.  min_p: null, or float32 [n_rows], and rows whose own is greater than 0 are left alone (egpt_sample_wide likewise).
+int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* uniform, int32_t* out, float* weights,
+                int n_rows, int vocab, const float* min_p, void* stream);
 // The same in stages for wide vocabularies (several workgroups per row, then the selection on the tokens that can still
 // be kept); workspace: egpt_sample_workspace(n_rows, vocab) bytes of device memory.
 size_t egpt_sample_workspace(int n_rows, int vocab);
 int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                     const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream);
+                     const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, const float* min_p, void* stream);
 // With a cut more (sampling_least.hip): min_p float32 [n_rows], of what top-k and top-p keep the tokens at least min_p times as likely as the
 // most likely one.  A row is cut into `pieces` <= 1,024 of at most 32,768 tokens (three fewer where rows begin between 16 bytes); workspace:
 // egpt_sample_min_p_workspace(n_rows, pieces) bytes of device memory, null for one piece.  Vocabularies below 2^23.
+// others: 0, or 1 where rows without a min_p of their own are left alone.
 size_t egpt_sample_min_p_workspace(int n_rows, int pieces);
 int egpt_sample_min_p(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                      const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, int pieces, void* stream);
+                      const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, int pieces, int others, void* stream);
 
 // ---- drafted tokens (attention_tree.hip, drafts.hip)
 // Attention for trees: operands as egpt_paged_attention; the last q_len[b] of a request's kv_len[b] tokens are its nodes.  visible int64

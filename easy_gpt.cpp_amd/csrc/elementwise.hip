@@ -773,4 +773,4 @@ extern "C" const char* egpt_error_string(int code) {
     }
 }
 
-extern "C" int egpt_abi_version(void) { return 30; }
+extern "C" int egpt_abi_version(void) { return 31; }

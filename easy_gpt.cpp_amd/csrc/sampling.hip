@@ -27,6 +27,9 @@ __global__ __launch_bounds__(kSampleThreads) void argmax_kernel(const float* __r
 // workgroup per row picks among the pieces (lowest index among equal maxima in both stages).
 constexpr int kArgmaxPieces = 32;
 
+// Of a call whose rows are not all sampled without min-p, those that have one (`min_p` not null) are another kernel's.
+__device__ __forceinline__ bool is_others(const float* __restrict__ min_p, int r) { return min_p && min_p[r] > 0.f; }
+
 // For sampling each wavefront leaves the maximum of its share as well (sub_val [rows][kSubPieces], -infinity where it had no
 // token).
 constexpr int kSubPieces = kArgmaxPieces * 4;
@@ -34,10 +37,11 @@ constexpr int kSubPieces = kArgmaxPieces * 4;
 __global__ __launch_bounds__(256) void argmax_pieces_kernel(const float* __restrict__ logits,
                                                             float* __restrict__ piece_val,
                                                             int32_t* __restrict__ piece_idx, float* __restrict__ sub_val,
-                                                            int vocab) {
+                                                            int vocab, const float* __restrict__ min_p) {
     __shared__ float s_val[16];
     __shared__ int s_idx[16];
     const int r = blockIdx.x, c = blockIdx.y;
+    if (is_others(min_p, r)) return;
     const int piece = (vocab + kArgmaxPieces - 1) / kArgmaxPieces;
     const int begin = min(vocab, c * piece), n = min(vocab, begin + piece) - begin;
     BestToken best{kNoToken, -INFINITY};
@@ -170,13 +174,14 @@ __global__ __launch_bounds__(256, 8) void sample_count_kernel(const float* __res
                                                           int32_t* __restrict__ list_count,
                                                           float* __restrict__ cand_w, int32_t* __restrict__ cand_idx,
                                                           unsigned int* __restrict__ piece_count,
-                                                          unsigned long long* __restrict__ piece_mass, int vocab) {
+                                                          unsigned long long* __restrict__ piece_mass, int vocab, const float* __restrict__ min_p) {
     __shared__ __attribute__((aligned(16))) float s_sub[kSubPieces];
     __shared__ unsigned int s_bound;
     __shared__ int s_n[2];
     __shared__ unsigned int s_count[kTopBins + 1];
     __shared__ unsigned long long s_mass[kTopBins + 1];
     const int r = blockIdx.x, c = blockIdx.y;
+    if (is_others(min_p, r)) return;
     const float temp = temperature[r];
     const int k = top_k[r];
     const bool by_count = k > 0 && k < vocab;
@@ -381,10 +386,11 @@ __global__ __launch_bounds__(256, 8) void sample_compact_kernel(const float* __r
                                                              unsigned long long* __restrict__ row_mass,
                                                              int32_t* __restrict__ direct_piece,
                                                              unsigned long long* __restrict__ direct_target,
-                                                             int32_t* __restrict__ last_bin, int vocab) {
+                                                             int32_t* __restrict__ last_bin, int vocab, const float* __restrict__ min_p) {
     __shared__ int s_wave[4];
     __shared__ SamplePlanSpace s_plan;
     const int r = blockIdx.x, c = blockIdx.y;
+    if (is_others(min_p, r)) return;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const float temp = temperature[r];
     if (!(temp > 0.f) || listed[r] != 0) {
@@ -612,7 +618,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     const float* __restrict__ top_p, const float* __restrict__ uniform, int32_t* __restrict__ out,
     float* __restrict__ weights, int vocab, const int32_t* __restrict__ cand_idx, const int32_t* __restrict__ cand_count,
     const int32_t* __restrict__ listed, const int32_t* __restrict__ list_count, const int32_t* __restrict__ best_in, const unsigned long long* __restrict__ row_mass,
-    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin) {
+    const int32_t* __restrict__ direct_piece, const unsigned long long* __restrict__ direct_target, const int32_t* __restrict__ last_bin,
+    const float* __restrict__ min_p) {
     __shared__ float s_val[16];
     __shared__ int s_idx[16];
     __shared__ unsigned int hist[256];
@@ -627,6 +634,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(
     __shared__ int s_pick[2];
     __shared__ __attribute__((aligned(16))) int s_order[kSampleThreads];
     const int r = blockIdx.x;
+    if (is_others(min_p, r)) return;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n_waves = blockDim.x / kWave;
     const float* row = logits + static_cast<size_t>(r) * vocab;
     float* w = weights + static_cast<size_t>(r) * vocab;
@@ -838,7 +846,7 @@ extern "C" int egpt_argmax(const float* logits, int32_t* out, void* scratch, int
     if (scratch && vocab >= 8192) {
         float* pv = static_cast<float*>(scratch);
         int32_t* pi = reinterpret_cast<int32_t*>(pv + static_cast<size_t>(n_rows) * kArgmaxPieces);
-        argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, nullptr, vocab);
+        argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, nullptr, vocab, nullptr);
         EGPT_CHECK_LAUNCH();
         argmax_pick_kernel<<<n_rows, kWave, 0, s>>>(pv, pi, out);
     } else {
@@ -885,14 +893,15 @@ extern "C" int egpt_argmax_static(const float* logits, int32_t* out, int n_rows,
     return egpt_argmax(logits, out, scratch, n_rows, vocab, stream);
 }
 
-// weights: scratch for n_rows * vocab floats.
-extern "C" int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                           const float* uniform, int32_t* out, float* weights, int n_rows, int vocab, void* stream) {
+// weights: scratch for n_rows * vocab floats.  min_p: null, or float32 [n_rows]; rows whose own is greater than 0 are left alone.
+extern "C" int egpt_sample(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* uniform, int32_t* out,
+                           float* weights, int n_rows, int vocab, const float* min_p, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !weights || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
     sample_kernel<<<n_rows, kSampleThreads, 0, static_cast<hipStream_t>(stream)>>>(
-        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+        logits, temperature, top_k, top_p, uniform, out, weights, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
+        min_p);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }
@@ -913,7 +922,7 @@ extern "C" size_t egpt_sample_workspace(int n_rows, int vocab) {
 }
 
 extern "C" int egpt_sample_wide(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p,
-                                const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, void* stream) {
+                                const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, const float* min_p, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !uniform || !out || !workspace || n_rows < 0 || vocab <= 0)
         return EGPT_BAD_ARGUMENT;
     if (n_rows == 0) return EGPT_OK;
@@ -936,17 +945,17 @@ extern "C" int egpt_sample_wide(const float* logits, const float* temperature, c
     float* sub = reinterpret_cast<float*>(p);                                  p += align256(r * kSubPieces * 4);
     float* pv = reinterpret_cast<float*>(p);
     int32_t* pi = reinterpret_cast<int32_t*>(pv + r * kArgmaxPieces);
-    argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, sub, vocab);
+    argmax_pieces_kernel<<<dim3(n_rows, kArgmaxPieces), 256, 0, s>>>(logits, pv, pi, sub, vocab, min_p);
     EGPT_CHECK_LAUNCH();
     sample_count_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, pv, pi, sub, best, listed, list_count, cand_w, cand_idx,
-                                                                    piece_count, piece_mass, vocab);
+                                                                    piece_count, piece_mass, vocab, min_p);
     EGPT_CHECK_LAUNCH();
     sample_compact_kernel<<<dim3(n_rows, kSamplePieces), 256, 0, s>>>(logits, temperature, top_k, top_p, uniform, best, piece_count,
                                                                       piece_mass, listed, cand_w, cand_idx, cand_count, row_mass,
-                                                                      direct_piece, direct_target, last_bin, vocab);
+                                                                      direct_piece, direct_target, last_bin, vocab, min_p);
     EGPT_CHECK_LAUNCH();
     sample_kernel<<<n_rows, kSampleThreads, 0, s>>>(logits, temperature, top_k, top_p, uniform, out, cand_w, vocab, cand_idx,
-                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin);
+                                                    cand_count, listed, list_count, best, row_mass, direct_piece, direct_target, last_bin, min_p);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }

@@ -427,9 +427,10 @@ __device__ __forceinline__ void pick_of_row(const float* __restrict__ row, int v
 template <int kQuads>
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_row_kernel(
     const float* __restrict__ logits, const float* __restrict__ temperature, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
-    const float* __restrict__ min_p, const float* __restrict__ uniform, int32_t* __restrict__ out, int vocab) {
+    const float* __restrict__ min_p, const float* __restrict__ uniform, int32_t* __restrict__ out, int vocab, int others) {
     __shared__ __attribute__((aligned(16))) LeastSpace s;
     const int r = blockIdx.x;
+    if (others && !(min_p[r] > 0.f)) return;
     const float* row = logits + static_cast<size_t>(r) * vocab;
     const int before = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 2 & 3u);
     float4 v[kQuads];
@@ -461,9 +462,10 @@ template <int kQuads>
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_pieces_kernel(
     const float* __restrict__ logits, const float* __restrict__ temperature, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
     const float* __restrict__ min_p, const float* __restrict__ uniform, int vocab, int quads_of_piece, PieceOfRow* __restrict__ found,
-    float* __restrict__ maxima, uint2* __restrict__ lists) {
+    float* __restrict__ maxima, uint2* __restrict__ lists, int others) {
     __shared__ __attribute__((aligned(16))) LeastSpace s;
     const int r = blockIdx.x, piece = blockIdx.y, pieces = gridDim.y;
+    if (others && !(min_p[r] > 0.f)) return;
     const size_t at = static_cast<size_t>(r) * pieces + piece;
     const float* row = logits + static_cast<size_t>(r) * vocab;
     const int before = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 2 & 3u);
@@ -491,9 +493,10 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_pieces_kernel(
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_joined_kernel(
     const float* __restrict__ logits, const float* __restrict__ temperature, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
     const float* __restrict__ min_p, const float* __restrict__ uniform, int32_t* __restrict__ out, int vocab, int pieces,
-    const PieceOfRow* __restrict__ found, const float* __restrict__ maxima, const uint2* __restrict__ lists) {
+    const PieceOfRow* __restrict__ found, const float* __restrict__ maxima, const uint2* __restrict__ lists, int others) {
     __shared__ __attribute__((aligned(16))) LeastSpace s;
     const int r = blockIdx.x, t = threadIdx.x, lane = t % kWave, wave = t / kWave;
+    if (others && !(min_p[r] > 0.f)) return;
     const size_t at = static_cast<size_t>(r) * pieces;
     // What may be asked for at once is: a piece to a thread, and of its wavefront's two first pieces an entry to a lane (where the piece listed so many).
     const int last = pieces - 1, shares = shares_of_piece(pieces);
@@ -558,7 +561,7 @@ extern "C" size_t egpt_sample_min_p_workspace(int n_rows, int pieces) {
 }
 
 extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                                 const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, int pieces, void* stream) {
+                                 const float* uniform, int32_t* out, void* workspace, int n_rows, int vocab, int pieces, int others, void* stream) {
     if (!logits || !temperature || !top_k || !top_p || !min_p || !uniform || !out || n_rows < 0 || vocab <= 0 || pieces < 1 || (pieces > 1 && !workspace))
         return EGPT_BAD_ARGUMENT;
     if (vocab >= 1 << 23 || pieces > kSampleThreads) return EGPT_UNSUPPORTED_SIZE;         // (masses in 64 bits, 40 behind the point)
@@ -570,8 +573,8 @@ extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, 
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool small = quads_of_piece <= 2 * kSampleThreads;
     if (pieces == 1) {
-        if (small) sample_row_kernel<2><<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab);
-        else sample_row_kernel<8><<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab);
+        if (small) sample_row_kernel<2><<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab, others);
+        else sample_row_kernel<8><<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab, others);
         EGPT_CHECK_LAUNCH();
         return EGPT_OK;
     }
@@ -582,7 +585,7 @@ extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, 
     uint2* lists = reinterpret_cast<uint2*>(at + whole_blocks(n * kMostShares * 4));
     const dim3 grid(n_rows, pieces);
     auto launch = [&](auto kernel) {
-        kernel<<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists);
+        kernel<<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists, others);
     };
     switch ((quads_of_piece + kSampleThreads - 1) / kSampleThreads) {       // (quads a thread)
         case 1:
@@ -594,7 +597,7 @@ extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, 
         default: launch(sample_pieces_kernel<8>);
     }
     EGPT_CHECK_LAUNCH();
-    sample_joined_kernel<<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab, pieces, found, maxima, lists);
+    sample_joined_kernel<<<n_rows, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, out, vocab, pieces, found, maxima, lists, others);
     EGPT_CHECK_LAUNCH();
     return EGPT_OK;
 }

@@ -32,11 +32,12 @@ Methods of a backend (T tokens, B requests, R rows, act = bfloat16 or float32):
   swiglu(gate_up act[T,2I], out act[T,I], activation='silu')   out = f(gate_up[:, :I]) * gate_up[:, I:], f silu or 'gelu_tanh', the
         tanh form of gelu (product_swiglu and gate_up_swiglu take the same)
   argmax(logits f32[R,V], out i32[R])            lowest index among equal maxima
-  sample(logits f32[R,V], temperature f32[R], top_k i32[R], top_p f32[R], uniform f32[R], out i32[R], min_p=None)
+  sample(logits f32[R,V], temperature f32[R], top_k i32[R], top_p f32[R], uniform f32[R], out i32[R], min_p=None, mixed=False)
         the weights exp((x - max) / temperature), cut to the top_k greatest (0 or V: all; ties whole), then to the fewest greatest
         whose mass reaches top_p (1: all; ties whole), then, with min_p f32[R] (0: all), to those of at least min_p times the
         greatest; the first token in index order whose running sum of what is left exceeds uniform * that sum; the lowest index of the
-        greatest where the temperature is 0 or less
+        greatest where the temperature is 0 or less.  mixed: rows whose min_p cuts nothing are sampled by the kernels of a call without min_p, and take its tokens,
+        which near a border of a cut or of the draw may be others (sums are rounded otherwise)
 
   tree_attention(qkv, out act[T,nq*hd], k_cache, v_cache, block_table i32[B,W], q_start i32[B], q_len i32[B], kv_len i32[B],
                  visible i64[T], nq, nkv, hd, page_size, scale, max_q_len, max_kv_len, window=0, positions=None)

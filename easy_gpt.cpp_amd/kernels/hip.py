@@ -31,7 +31,7 @@ def _load_library() -> ctypes.CDLL:
         lib = ctypes.CDLL(path)
     except (build.BuildError, OSError) as e:
         raise KernelsUnavailable(f"the HIP kernel library could not be built or loaded: {e}") from e
-    if lib.egpt_abi_version() != 30:
+    if lib.egpt_abi_version() != 31:
         raise KernelsUnavailable(f"{path} has an unexpected ABI version")
     return lib
 
@@ -109,9 +109,9 @@ class HipKernels(KernelBackend):
             "egpt_attention_any_tiled": [vp, vp, vp, vp, vp, i, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_attention_any_decode": [vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i, i, i, i, i, f, i, i, i, vp],
             "egpt_argmax": [vp, vp, vp, i, i, vp],
-            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
-            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
-            "egpt_sample_min_p": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp],
+            "egpt_sample": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp],
+            "egpt_sample_wide": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp],
+            "egpt_sample_min_p": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
             "egpt_tree_attention_generic": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, vp],
             "egpt_tree_attention": [vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, i, i, i, i, i, vp],
             "egpt_accept_drafts": [vp, vp, vp, vp, vp, i, i, vp, vp, vp, vp],
@@ -2196,8 +2196,10 @@ class HipKernels(KernelBackend):
     def _sample_space(self, rows: int, pieces: int) -> int:
         return int(self.lib.egpt_sample_min_p_workspace(rows, pieces))
 
-    def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None):
+    def sample(self, logits, temperature, top_k, top_p, uniform, out, min_p=None, mixed=False):
         r, v = logits.shape
+        if mixed and min_p is None:
+            raise ValueError("mixed needs min_p, which says which rows are sampled without it")
         if min_p is not None:
             self._here(logits, "logits", _F32)
             device = logits.get_device()
@@ -2207,8 +2209,9 @@ class HipKernels(KernelBackend):
                 pieces = self._sample_pieces(r, v, v % 4 == 0 and logits.data_ptr() % 16 == 0)
                 space = torch.empty(self._sample_space(r, pieces), dtype=torch.uint8, device=logits.device) if pieces > 1 else None
                 self._run("egpt_sample_min_p", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
-                          uniform.data_ptr(), out.data_ptr(), self._ptr(space), r, v, pieces, self._stream())
-            return
+                          uniform.data_ptr(), out.data_ptr(), self._ptr(space), r, v, pieces, int(mixed), self._stream())
+            if not mixed:
+                return
         self._need(logits, "logits", _F32)
         self._need(temperature, "temperature", _F32, (r,))
         self._need(top_k, "top_k", _I32, (r,))
@@ -2219,11 +2222,11 @@ class HipKernels(KernelBackend):
             # a wide vocabulary: the row-wide passes by many workgroups, the selection on the tokens that are left
             space = torch.empty(int(self.lib.egpt_sample_workspace(r, v)), dtype=torch.uint8, device=logits.device)
             self._run("egpt_sample_wide", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
-                      uniform.data_ptr(), out.data_ptr(), space.data_ptr(), r, v, self._stream())
+                      uniform.data_ptr(), out.data_ptr(), space.data_ptr(), r, v, self._ptr(min_p), self._stream())
             return
         weights = torch.empty((r, v), dtype=_F32, device=logits.device)
         self._run("egpt_sample", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
-                  uniform.data_ptr(), out.data_ptr(), weights.data_ptr(), r, v, self._stream())
+                  uniform.data_ptr(), out.data_ptr(), weights.data_ptr(), r, v, self._ptr(min_p), self._stream())
 
     # ------------------------------------------------------------------ drafted tokens
     # (Calls whose kernels take a few microseconds: what is usual is told by a few cheap questions, the rest is left to the careful ones.)

@@ -119,6 +119,8 @@ class Sampler:
             # would: with a step launched ahead, that is the step whose tokens are not needed yet)
             pinned = logits.is_cuda
             least = any(p.min_p > 0 and not p.greedy for p in params)
+            # (a request without min-p has the tokens, and its kernels the time, that they have without a neighbour that uses it)
+            mixed = least and any(p.min_p == 0 and not p.greedy for p in params)
             host = torch.empty((5 if least else 4, r), dtype=torch.float32, pin_memory=pinned)
             rows = host.numpy()
             rows[0] = [0.0 if p.greedy else p.temperature for p in params]
@@ -128,5 +130,6 @@ class Sampler:
             if least:
                 rows[4] = [p.min_p for p in params]
             dev = host.to(logits.device, non_blocking=pinned)
-            k.sample(logits, dev[0], dev[3].view(torch.int32), dev[1], dev[2], out, **({"min_p": dev[4]} if least else {}))
+            k.sample(logits, dev[0], dev[3].view(torch.int32), dev[1], dev[2], out, **({"min_p": dev[4]} if least else {}),
+                     **({"mixed": True} if mixed else {}))
         return PendingTokens(out)

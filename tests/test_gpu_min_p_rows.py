@@ -57,3 +57,60 @@ def test_masked_rows_take_no_longer(mask, cuts):
     assert got == out.tolist()                               # (the tokens of the row without what is masked)
     print(f"cuts {cuts} mask {mask}: {here:.1f} us, unmasked {whole:.1f}")
     assert here < 1.4 * whole
+
+
+def border_uniforms(x, temperature, top_k, g):
+    """For every row a uniform number that falls, to the last bit or next to it, on the running sum of the tokens that top-k leaves."""
+    w = torch.exp((x - x.max(1, keepdim=True).values) / temperature)
+    if top_k:
+        w = torch.where(w >= torch.topk(w, top_k).values[:, -1:], w, torch.zeros_like(w))
+    share = torch.cumsum(w.double(), 1)
+    share /= share[:, -1:]
+    return share.gather(1, torch.randint(0, x.shape[1] - 1, (x.shape[0], 1), generator=g).to(x.device))[:, 0].float()
+
+
+@pytest.mark.parametrize("vocab,top_k", [(700, 0), (700, 20), (5000, 20), (5000, 0), (40000, 50), (40000, 0)])
+def test_a_request_has_the_tokens_that_it_has_without_a_neighbour_with_min_p(monkeypatch, vocab, top_k):
+    from easy_gpt.cpp_amd.sampling import Sampler, SamplingParams, sampler
+
+    rows, g = 512, torch.Generator().manual_seed(vocab + top_k)
+    x = (torch.randn((rows, vocab), generator=g) * 1.5).to(DEV)
+    u = border_uniforms(x, 0.9, top_k, g).cpu().numpy()
+
+    def uniforms(params, serials, counts, out):
+        out[:] = u
+
+    monkeypatch.setattr(sampler, "fill_uniforms", uniforms)
+    plain = [SamplingParams(temperature=0.9, top_k=top_k, top_p=1.0 if r % 3 else 0.9) for r in range(rows)]
+    with_one = [SamplingParams(temperature=0.9, top_k=top_k, top_p=p.top_p, min_p=0.05) if r in (3, 200) else p for r, p in enumerate(plain)]
+    s, numbers = Sampler(DEV), list(range(rows))
+    alone, beside = s.sample(x, plain, numbers, numbers), s.sample(x, with_one, numbers, numbers)
+    assert [r for r in numbers if alone[r] != beside[r] and r not in (3, 200)] == []
+    # and the two have the tokens that they have among their like
+    among = s.sample(x, [SamplingParams(temperature=0.9, top_k=top_k, top_p=p.top_p, min_p=0.05) for p in plain], numbers, numbers)
+    assert beside[3] == among[3] and beside[200] == among[200]
+
+
+@pytest.mark.parametrize("top_k,top_p", [(0, 0.95), (0, 1.0), (50, 0.95)])
+def test_a_neighbour_with_min_p_costs_its_own_time(monkeypatch, top_k, top_p):
+    # 64 rows of 151,936, one of them with min-p: the kernels of the other 63 and those of one row (7 to 20 us) behind each other
+    from easy_gpt.cpp_amd.sampling import Sampler, SamplingParams
+
+    rows, vocab = 64, 151936
+    x = (torch.randn((rows, vocab), generator=torch.Generator().manual_seed(3)) * 2.5).to(DEV)
+    k, asked = kernels.backend(), []
+    sample = type(k).sample
+    monkeypatch.setattr(k, "sample", lambda *a, **kw: asked.append((a, kw)) or sample(k, *a, **kw), raising=False)
+    one = SamplingParams(temperature=1.0, top_k=top_k, top_p=top_p)
+    other = SamplingParams(temperature=1.0, top_k=top_k, top_p=top_p, min_p=0.05)
+    s, numbers = Sampler(DEV), list(range(rows))
+    s.sample(x, [one] * rows, numbers, numbers)
+    s.sample(x, [one] * 20 + [other] + [one] * 43, numbers, numbers)
+    alone, beside = (microseconds(lambda: sample(k, *a, **kw)) for a, kw in asked)
+    print(f"top-k {top_k} top-p {top_p}: {alone:.1f} us, beside one with min-p {beside:.1f}")
+    assert beside < 1.05 * alone + 20
+
+
+def test_mixed_calls_are_refused_without_min_p():
+    with pytest.raises(ValueError):
+        kernels.backend().sample(torch.zeros((2, 9), device=DEV), *operands(2, 1.0, 0, 1.0, 0.1)[:5], mixed=True)
