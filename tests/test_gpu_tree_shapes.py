@@ -156,3 +156,129 @@ def test_windows_that_32_bits_do_not_hold_are_refused(window):
     c["window"] = window
     with pytest.raises(ValueError):
         run_shape(pytest.MonkeyPatch(), c, 14, 1)
+
+
+def check(monkeypatch, c, shape, parts, oracle=None):
+    """Against 64 bits; rows of no request stay.  Twice, to the same bits."""
+    want, spread = expected(oracle or c)
+    got = run_shape(monkeypatch, c, shape, parts)
+    nobody = want.isnan()
+    assert bool(got.cpu()[nobody].isnan().all())
+    tol = plain.tree_tolerance(c, spread, want)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol)[~nobody].all()), float((err / tol)[~nobody].max())
+    again = run_shape(monkeypatch, c, shape, parts)
+    assert torch.equal(again.nan_to_num(9.0), got.nan_to_num(9.0))
+    return got
+
+
+@in_parts
+@every_shape
+def test_uneven_trees(monkeypatch, dtype, hd, shape, parts):
+    # from one row to more than a workgroup has, behind none to many rounds of keys, empty requests among them; seven query heads to a kv head, so that rows do not fill blocks
+    c, _ = plain.tree_case(random.Random(51), [1, 0, 64, 13, 40, 2], [0, 50, 1100, 333, 64, 17], 14, 2, hd, 16, dtype, DEV, extra_rows=3)
+    check(monkeypatch, c, shape, parts)
+
+
+@in_parts
+@pytest.mark.parametrize("less", [16, 8], ids=["16_less", "half"])
+@every_shape
+def test_heads_that_do_not_fill_the_instance(monkeypatch, dtype, hd, shape, parts, less):
+    # (that of 64 takes 8 to 64 features, that of 128 up to 128 and so on)
+    mine = hd - 16 if less == 16 else hd // 2 + 8
+    c, _ = plain.tree_case(random.Random(52), [9, 33], [70, 700], 4, 2, mine, 32, dtype, DEV)
+    check(monkeypatch, c, shape, parts)
+
+
+@in_parts
+@pytest.mark.parametrize("window", [1, 40, 600])
+@every_shape
+def test_windows(monkeypatch, dtype, hd, shape, parts, window):
+    c, _ = plain.tree_case(random.Random(53), [20, 64, 1], [1333, 150, 40], 4, 2, hd, 16, dtype, DEV, window=window)
+    c["block_table"][0, : max(0, 1333 - window) // 16] = -1  # (what lies behind all windows was given back)
+    check(monkeypatch, c, shape, parts)
+
+
+@in_parts
+@every_shape
+def test_any_set_of_nodes_and_rows_that_see_nothing(monkeypatch, dtype, hd, shape, parts):
+    c, _ = plain.tree_case(random.Random(54), [64, 40], [300, 0], 4, 2, hd, 16, dtype, DEV)
+    rng = random.Random(55)
+    c["visible"][:64] = torch.tensor([rng.getrandbits(64) - (1 << 63) for _ in range(64)], dtype=torch.int64, device=DEV)
+    c["visible"][64:] = torch.tensor([0 if i % 3 == 0 else 1 << (i % 40) for i in range(40)], device=DEV)
+    c["visible"][65] = -1 << 40                              # only nodes that the request does not have
+    got = check(monkeypatch, c, shape, parts)
+    assert not bool(got[64].any()) and not bool(got[65].any())
+
+
+@in_parts
+@every_shape
+def test_missing_pages(monkeypatch, dtype, hd, shape, parts):
+    c, _ = plain.tree_case(random.Random(56), [12, 7], [1500, 200], 4, 2, hd, 16, dtype, DEV)
+    c["v_cache"] += 3.0
+    c["block_table"][:, 3] = -1
+    c["block_table"][0, [60, 61, 80]] = -1
+    oracle = dict(c, block_table=c["block_table"].clone())
+    c["block_table"][0, 33], oracle["block_table"][0, 33] = c["k_cache"].shape[0], -1
+    check(monkeypatch, c, shape, parts, oracle)
+
+
+@in_parts
+@pytest.mark.parametrize("number", [math.inf, -math.inf, math.nan])
+@every_shape
+def test_numbers_in_unseen_nodes(monkeypatch, dtype, hd, shape, parts, number):
+    # node 3 of 12 holds no finite numbers: rows that do not see it are as if it held others; rows that do are as finite as the formula's
+    c, _ = plain.tree_case(random.Random(57), [12, 5], [445, 20], 4, 2, hd, 16, dtype, DEV)
+    place = 445 + 3
+    page = int(c["block_table"][0, place // 16])
+    c["v_cache"][page, :, : hd // 2, place % 16] = number
+    c["k_cache"][page, 1, place % 16, 0] = number
+    sees = torch.tensor([b >> 3 & 1 for b in c["visible"].tolist()[:12]] + [0] * 5, dtype=torch.bool)
+    assert 0 < int(sees.sum()) < 12
+    clean = dict(c, v_cache=c["v_cache"].clone(), k_cache=c["k_cache"].clone())
+    clean["v_cache"][page, :, :, place % 16] = 0.5
+    clean["k_cache"][page, :, place % 16] = 0.5
+    got = run_shape(monkeypatch, c, shape, parts).cpu().double()
+    want, spread = expected(clean)
+    tol = plain.tree_tolerance(clean, spread, want)
+    assert bool(((got - want).abs() <= tol)[~sees].all())
+    assert torch.equal(got[sees].isfinite(), expected(c)[0][sees].isfinite())
+
+
+@in_parts
+@every_shape
+def test_infinities_before_the_tree(monkeypatch, dtype, hd, shape, parts):
+    c, _ = plain.tree_case(random.Random(58), [9], [700], 2, 1, hd, 16, dtype, DEV)
+    c["v_cache"][int(c["block_table"][0, 20]), 0, 3, 5] = math.inf
+    got = run_shape(monkeypatch, c, shape, parts).cpu().float().view(9, 2, hd)
+    assert bool((got[:, :, 3] == math.inf).all())
+    assert bool(got[:, :, :3].isfinite().all()) and bool(got[:, :, 4:].isfinite().all())
+
+
+@in_parts
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@every_shape
+def test_any_scale(monkeypatch, dtype, hd, shape, parts, scale):
+    c, _ = plain.tree_case(random.Random(59), [9, 4], [570, 3], 4, 2, hd, 16, dtype, DEV, spread=0.5)
+    c["scale"] = scale
+    check(monkeypatch, c, shape, parts)
+
+
+@pytest.mark.parametrize("parts", [2, 7, 64])
+@every_shape
+def test_a_long_context_in_any_number_of_parts(monkeypatch, dtype, hd, shape, parts):
+    c, _ = plain.tree_case(random.Random(60), [24, 3], [4000, 900], 4, 2, hd, 16, dtype, DEV)
+    check(monkeypatch, c, shape, parts)
+
+
+def test_the_rule_chooses_every_shape():
+    # (what the tests above ask for by name is what some sizes get)
+    k = kernels.backend()
+    chosen = set()
+    for dt, size in ((1, 64), (1, 128), (1, 256), (0, 64), (0, 128), (0, 256)):
+        for b in (1, 2, 8, 64):
+            for n in (1, 8, 16, 32, 64):
+                for group in (1, 7, 14):
+                    for kv in (64, 512, 4096, 32768):
+                        chosen.add((dt, size, k._tree_shape(b, b * n, 2, group, size, dt, n, kv)[0]))
+    assert chosen == {(int(d is BF16), h, s) for d, h, s in SHAPES}
