@@ -17,8 +17,8 @@ __global__ __launch_bounds__(64) void accept_drafts_kernel(const int32_t* __rest
                                                            const int32_t* __restrict__ q_len, int n_tokens, int32_t* __restrict__ path,
                                                            int32_t* __restrict__ count, int32_t* __restrict__ accepted) {
     const int b = blockIdx.x, lane = threadIdx.x;
-    const int at = q_start[b], n = min(q_len[b], kTreeNodes);
-    const bool here = lane < n && at >= 0 && lane < n_tokens - at;
+    const int at = q_start[b], n = at >= 0 && at < n_tokens ? min(q_len[b], kTreeNodes) : 0;         // (one that begins nowhere has no nodes)
+    const bool here = lane < n && lane < n_tokens - at;
     const int token = here ? tokens[at + lane] : -1, parent = here ? parents[at + lane] : -1, next = here ? sampled[at + lane] : -1;
     int length = 0, mine = -1;
     if (n > 0) {

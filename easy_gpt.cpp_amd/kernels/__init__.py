@@ -51,7 +51,7 @@ Methods of a backend (T tokens, B requests, R rows, act = bfloat16 or float32):
         the walk through a tree whose node 0 is the token sampled last and whose node i > 0 drafts tokens[i] behind node
         parents[i] < i: from the root to the child whose token is what the model sampled behind its parent (the lowest of several) until there is
         none.  path: the nodes passed, the root among them, count of them; accepted: what was sampled behind each, the request's
-        new tokens; -1 behind the last
+        new tokens; -1 behind the last.  A request without nodes, or that begins at no token, takes none
   keep_drafts(k_cache [slabs,P,nkv,page_size,dk] | [P,...], v_cache [slabs,P,nkv,dv,page_size] | [P,...], block_table i32[B,W],
               start i32[B], path i32[B,L], count i32[B])
         key and value of the first count[b] nodes of an ascending path, which lie at places start[b] + path[b,k] of their request, go to places
