@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_attention_generic_kernel
 //
 // A head beyond 128 is more registers of queries and sums than a wavefront has: two share a block of rows, each with half of the features, and add up their halves of
 // the scores through LDS, one barrier more a tile (float32, 7 requests of one node behind 1,246 tokens at 12 heads on 2 of 256: 71.6 us by one wavefront with its
-// registers in memory, 29.0 so, and half the rounding error).
+// registers in memory, 28 so, and half the rounding error).
 //
 // A request's keys are cut into parts, a workgroup each, so that few requests fill the card and a long context does not make the others wait;
 // parts leave the unnormalised result with its maximum and sum, and tree_combine_kernel joins them.

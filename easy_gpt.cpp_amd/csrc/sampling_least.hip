@@ -458,11 +458,12 @@ struct PieceOfRow {
 __device__ __forceinline__ int shares_of_piece(int pieces) { return pieces <= 16 ? 64 : pieces <= 32 ? 32 : 16; }
 constexpr int kMostShares = 64;
 
+// (what is asked for first stands in the arguments that arrive with the wavefronts)
 template <int kQuads>
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_pieces_kernel(
     const float* __restrict__ logits, const float* __restrict__ temperature, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
-    const float* __restrict__ min_p, const float* __restrict__ uniform, int vocab, int quads_of_piece, PieceOfRow* __restrict__ found,
-    float* __restrict__ maxima, uint2* __restrict__ lists, int others) {
+    const float* __restrict__ min_p, int vocab, int quads_of_piece, int others, const float* __restrict__ uniform, PieceOfRow* __restrict__ found,
+    float* __restrict__ maxima, uint2* __restrict__ lists) {
     __shared__ __attribute__((aligned(16))) LeastSpace s;
     const int r = blockIdx.x, piece = blockIdx.y, pieces = gridDim.y;
     if (others && !(min_p[r] > 0.f)) return;
@@ -585,7 +586,7 @@ extern "C" int egpt_sample_min_p(const float* logits, const float* temperature, 
     uint2* lists = reinterpret_cast<uint2*>(at + whole_blocks(n * kMostShares * 4));
     const dim3 grid(n_rows, pieces);
     auto launch = [&](auto kernel) {
-        kernel<<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, uniform, vocab, quads_of_piece, found, maxima, lists, others);
+        kernel<<<grid, kSampleThreads, 0, st>>>(logits, temperature, top_k, top_p, min_p, vocab, quads_of_piece, others, uniform, found, maxima, lists);
     };
     switch ((quads_of_piece + kSampleThreads - 1) / kSampleThreads) {       // (quads a thread)
         case 1:

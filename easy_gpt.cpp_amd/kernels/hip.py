@@ -2185,7 +2185,9 @@ class HipKernels(KernelBackend):
         rows begin between 16 bytes), by one launch; a longer row is of pieces of 8,192 as long as those of all rows are about as many as there are
         compute units, then of 20,480, and of 32,768 where there are many rows anyway (tokens of 151,936, us with 19, with 8 and with 5 pieces a
         row: 1 row 7.6, 8.2 and 9.6, 32 rows 14.1, 12.1 and 14.0, 64 rows 15.9, 14.7 and 16.5, 1,024 rows 179, 130 and 126; of 32,768 with 5
-        pieces and with 1: 1 row 9.1 and 7.5, 256 rows 19.3 and 10.3)."""
+        pieces and with 1: 1 row 9.1 and 7.5, 256 rows 19.3 and 10.3).  With other vocabularies the rule is at most 8 % slower than the best of the three (by
+        top-k, top-p and min-p; of 65,536 with 8, 4 and 2 pieces 1 row 10.5, 11.3 and 11.9, 64 rows 14.4, 13.2 and 14.3, 1,024 rows 86.8, 61.9 and 64.4; of
+        200,000 with 25, 10 and 7 1 row 12.6, 13.1 and 14.1, 32 rows 19.9, 16.3 and 15.1, 1,024 rows 262, 168 and 163)."""
         off = 0 if aligned else 3
         if vocab <= 32768 - off:
             return 1
