@@ -42,7 +42,7 @@ USAGE = """Usage: easy_llm [--model <dir>] [--prompt-file <path>] [--max-steps <
       --cache-tokens <n>     Tokens the paged cache holds (default: 65536)
       --page-size <n>        Tokens per cache page (default: 16)
       --draft-nodes <n>      Tokens that a step checks for a decoding request, up to 64: its last one and what its own
-                             tokens say may follow (default: 0, the last one alone)
+                             tokens say may follow; for few requests whose text repeats (default: 0, the last one alone)
       --tune-products        Choose the library's matrix products by measurement (about a second per new shape)
   -h, --help                Show this help message
 Examples:

@@ -8,8 +8,8 @@
 // infinity or a NaN.
 //
 // What bounds it, on the device alone: few rows, the chain of memory trips, a few rounds of keys and the join of the parts (1 user of 8 nodes behind 301 tokens at 14 heads on 2 of
-// 64 7.1 us, 8 users of 16 behind 2,048 at 12 heads on 2 of 128 15.9); rows of small heads, the vector instructions of the softmax (64 users of 1 to 32
-// nodes behind 128 to 4,001 at 14 heads on 2 of 64 32.8, 2.3 TB/s of keys and values); many rows, the matrix cores and the softmax, which overlap for a quarter of
+// 64 7.1 us, 8 users of 16 behind 2,048 at 12 heads on 2 of 128 15.7); rows of small heads, the vector instructions of the softmax (64 users of 1 to 32
+// nodes behind 128 to 4,001 at 14 heads on 2 of 64 32.6, 2.3 TB/s of keys and values); many rows, the matrix cores and the softmax, which overlap for 37 % of
 // the products' time (2 users of 64 nodes behind 32,001 at 28 heads on 4 of 128 78, 750 TFLOP/s, where a library product reaches 1,400).
 #include <atomic>
 #include <type_traits>

@@ -4,13 +4,14 @@
 // that needs no search and leaves a few dozen tokens of a model's distribution.  So a row is read once, into the registers of one workgroup or, a long one,
 // of several: the greatest logit is known behind one barrier, the tokens that reach the bound below it go to a list.  Top-k needs the k-th
 // largest weight: the k-th largest of the threads' own maxima is no larger, and stands in the same comparison.  Top-p without top-k refers to the
-// mass of the whole row, added up from the registers too.  All cuts and the draw then run on the list, as searches for the bin that holds a count or a mass.
+// mass of the whole row, added up from the registers too, in 32 bits a thread and 64 beyond: which tokens within some 2^-18 of top_p are kept may go by the
+// number of pieces (integers would need the row's maximum first, or the row twice).  All cuts and the draw then run on the list, as searches for the bin that holds a count or a mass.
 // A row in pieces leaves a list, a maximum and a mass for each, and a second kernel joins them: the pieces' bounds are lower than the row's, so their
 // lists hold what the row's does.  Rows that leave too long a list (nearly flat ones; top-p alone with a min_p of 0) are walked again for each threshold.
 //
-// What bounds it: for many rows the one pass over the logits (1,024 rows of 32,768 with top-p and min-p: 30.2 us, 4.4 TB/s, where a copy reaches 5.1;
+// What bounds it: for many rows the one pass over the logits (1,024 rows of 32,768 with top-p and min-p: 29.7 us, 4.5 TB/s, where a copy reaches 5.1;
 // 254 by the kernels that count and list in passes of their own, with a workgroup's list of hundreds compared pair by pair); for a few the chain of a load, a
-// dozen barriers and a second launch (1 row of 151,936 7.6 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 19.1).
+// dozen barriers and a second launch (1 row of 151,936 7.8 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 19.2).
 // Rows without a usable bound: 64 of 151,936 with top-p alone 263 us, a min_p of 10^-6 45.
 #include "api.h"
 #include "common.h"

@@ -3,8 +3,8 @@
 Text repeats itself (quotations, code, lists, names): where the last few tokens stood before, what followed them then is a
 guess at what follows now.  `PromptLookup` keeps, per request, the places of every run of 1 to `longest` tokens and proposes
 the continuations behind the latest places of the longest run that has any, as a tree whose root is the last token.  A guess
-costs nothing but rows of the step that checks it (`Engine.step_drafts`): what the model does not say itself is dropped, so the
-tokens of a request are those that it has without drafts.
+costs rows of the step that checks it (`Engine.step_drafts`): what the model does not say itself is dropped, so the
+tokens of a request are those that it has without drafts, up to the rounding of a step with more rows (in float32 the last bits).
 
 The reference decodes one token per request and step (/root/reference/src/continuous_batch_server.cpp:160-212).
 """

@@ -310,7 +310,8 @@ class Engine:
         says what follows each node (rows in the order of the entries and of their nodes), and every request takes the path from its root
         along the nodes that were chosen (`accept_drafts`).  Returns each request's new tokens, what was chosen behind the nodes of the
         path: one at least.  The path's keys and values become the request's; the other nodes leave nothing.  A token
-        is what it would be one step at a time, as far as `choose` says the same of the same logits.  Raises OutOfPages (with the
+        is what it would be one step at a time, as far as `choose` says the same of these logits, which are those of such a step up to
+        rounding (of bfloat16; in float32 the last bits, as sums are taken in another order).  Raises OutOfPages (with the
         cache unchanged) if the nodes do not fit."""
         from .. import kernels
 

@@ -10,8 +10,10 @@ prompt portions in arrival order.
 
 With drafts (`SchedulerConfig.draft_nodes`) a step in which every entry decodes checks, beside each request's last token, what its
 own tokens say may follow (`engine.drafting`), and a request may gain several tokens from it; the tokens are those that it would
-have without, since the uniform number of its n-th token is the same either way (bfloat16 rounds the logits of a step with more rows
-otherwise, as for any batch).  Steps then wait for each other.
+have without, up to rounding: the uniform number of its n-th token is the same either way, its logits are summed up in another order (in
+float32 they differ in the last bits, in bfloat16 as in any batch of more rows).  A step with a portion of a prompt drafts
+nothing, and no step is launched ahead, also where nothing was drafted.  One user whose text repeats gains; many users lose more by their
+steps, which take the products of prompts and wait for each other, than accepted tokens give.
 
 Decoding runs one step ahead of the host where it can: while a decode step is on the GPU, the next one (the same
 requests, one token each) is launched behind it with its token ids taken on the device from what the sampler leaves

@@ -45,7 +45,8 @@ class LLM:
         draft_nodes: int = 0,
     ):
         """draft_nodes: tokens that a step checks for a decoding request, its last one and what its own tokens say may follow
-        (`engine.PromptLookup`); up to 64, 0 or 1: the last one alone."""
+        (`engine.PromptLookup`); up to 64, 0 or 1: the last one alone.  For one user, or few, whose text repeats itself: steps of
+        drafts wait for each other and take longer than a decode step."""
         self.engine = Engine.from_dir(model_dir, dtype=dtype, device=device, page_size=page_size,
                                       max_tokens=cache_tokens, max_requests=max_active, tune_products=tune_products,
                                       allow_unexpected_tensors=allow_unexpected_tensors)

@@ -6,7 +6,7 @@ takes the first maximum; otherwise probabilities are raised to 1/T (softmax(logi
 cut to the top_k most likely (0 disables), then to the smallest set whose mass reaches
 top_p (1 disables), and one uniform number picks a token from what is left.  min_p, which the
 reference does not have, then drops the tokens less than min_p times as likely as the most likely
-one (0 disables).
+one (0 disables).  In a batch where only some requests have it the others are sampled as without it.
 
 The reference draws from one shared mt19937 in batch order, so a request's tokens
 depend on its neighbours.  Here the uniform number of a request's n-th token is a
