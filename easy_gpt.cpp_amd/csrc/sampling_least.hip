@@ -4,8 +4,8 @@
 // that needs no search and leaves a few dozen tokens of a model's distribution.  So a row is read once, into the registers of one workgroup or, a long one,
 // of several: the greatest logit is known behind one barrier, the tokens that reach the bound below it go to a list.  Top-k needs the k-th
 // largest weight: the k-th largest of the threads' own maxima is no larger, and stands in the same comparison.  Top-p without top-k refers to the
-// mass of the whole row, added up from the registers too, in 32 bits a thread and 64 beyond: which tokens within some 2^-18 of top_p are kept may go by the
-// number of pieces (integers would need the row's maximum first, or the row twice).  All cuts and the draw then run on the list, as searches for the bin that holds a count or a mass.
+// mass of the whole row, added up from the registers too, in 32 bits a thread and 64 beyond; where that leaves in doubt which tokens reach top_p, the row is
+// walked with masses in integers, as the kernels without min-p have them.  All cuts and the draw then run on the list, as searches for the bin that holds a count or a mass.
 // A row in pieces leaves a list, a maximum and a mass for each, and a second kernel joins them: the pieces' bounds are lower than the row's, so their
 // lists hold what the row's does.  Rows that leave too long a list (nearly flat ones; top-p alone with a min_p of 0) are walked again for each threshold.
 //
@@ -79,7 +79,7 @@ struct LeastSpace {
     unsigned long long mass[2][kBins];
     unsigned int count[2][kBins];
     double row_mass[kWaves];
-    unsigned long long sums[kWaves * 15], above, need;
+    unsigned long long sums[kWaves * 15], above, within, need;
     unsigned int hist[256], needed;
     float k_bound;
     float best_val[kWaves];
@@ -107,8 +107,9 @@ __device__ __forceinline__ unsigned long long sum_up_to(unsigned long long v) {
 // Among the list's entries the greatest key of [lo, hi) whose mass with that of all greater keys reaches what need_of makes of the mass of all; lo if none
 // does.  entry(j, key, mass): whether the j-th takes part (asked by the thread that has it, j modulo the threads).  Masses are integers, whose
 // sums depend on no order.  Left in lo and hi: the bin of the last pass, which holds that key and no other.  Every pass counts 256 bins; few
-// entries need more than two.  One set of bins is cleared while the other is looked at: `turn`, the one that is clear.
-template <typename Entry, typename Need>
+// entries need more than two.  One set of bins is cleared while the other is looked at: `turn`, the one that is clear.  BORDERS: the masses of all greater keys
+// and of that key are left in s.above and s.within (where none reaches the need, the mass of all, and more than any need).
+template <bool BORDERS, typename Entry, typename Need>
 __device__ __forceinline__ void bound_in_list(int n, Entry entry, uint32_t& lo, uint32_t& hi, Need need_of, int& turn, LeastSpace& s) {
     const int lane = threadIdx.x % kWave;
     unsigned long long above = 0ull;
@@ -133,23 +134,34 @@ __device__ __forceinline__ void bound_in_list(int n, Entry entry, uint32_t& lo, 
             for (int i = 0; i < 4; ++i) sum += mine[i] = masses[top - i];
             const unsigned long long incl = sum_up_to(sum);
             unsigned long long need = s.need;
-            if (first) need = need_of(static_cast<unsigned long long>(__builtin_amdgcn_readlane(static_cast<uint32_t>(incl >> 32), kWave - 1)) << 32 |
-                                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(incl), kWave - 1)));
+            unsigned long long all = 0ull;
+            if (first) {
+                all = static_cast<unsigned long long>(__builtin_amdgcn_readlane(static_cast<uint32_t>(incl >> 32), kWave - 1)) << 32 |
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(incl), kWave - 1));
+                need = need_of(all);
+            }
             const unsigned long long reached = __ballot(above + incl >= need);
             if (lane == (reached ? __ffsll(static_cast<long long>(reached)) - 1 : 0)) {
                 s.need = need;
                 s.done = 1;
                 s.lo = lo;
                 s.hi = hi;
+                if constexpr (BORDERS) {                     // (for as long as nothing reaches it: in the first pass or never)
+                    s.above = all;
+                    s.within = 1ull << 63;
+                }
                 if (reached) {
                     unsigned long long cum = above + incl - sum;
+                    [[maybe_unused]] unsigned long long within = mine[0];
                     int bin = top;
 #pragma unroll
                     for (int i = 0; i < 3; ++i)
                         if (bin == top - i && cum + mine[i] < need) {
                             cum += mine[i];
+                            within = mine[i + 1];
                             --bin;
                         }
+                    if constexpr (BORDERS) s.within = within;
                     s.lo = lo + (static_cast<uint32_t>(bin) << shift);
                     s.hi = min(hi, lo + (static_cast<uint32_t>(bin + 1) << shift));
                     s.above = cum;
@@ -376,13 +388,19 @@ __device__ __forceinline__ void pick_of_row(const float* __restrict__ row, int v
         threshold = least_listed;
         uint32_t hi = kTop;
         if (c.by_count) {
-            bound_in_list(listed, [&](int j, uint32_t& key, unsigned long long& mass) { key = s.w[j]; mass = 1ull; return true; }, threshold, hi,
-                          [&](unsigned long long) { return static_cast<unsigned long long>(c.k); }, turn, s);
+            bound_in_list<false>(listed, [&](int j, uint32_t& key, unsigned long long& mass) { key = s.w[j]; mass = 1ull; return true; }, threshold, hi,
+                                 [&](unsigned long long) { return static_cast<unsigned long long>(c.k); }, turn, s);
             hi = kTop;
         }
+        bool sure = true;
         if (c.by_mass) {
-            bound_in_list(listed, [&](int j, uint32_t& key, unsigned long long& mass) { key = s.w[j]; mass = fixed_of(__uint_as_float(key)); return true; },
-                          threshold, hi, [&](unsigned long long all) { return needed_mass(c.p, c.by_count ? all : row_mass); }, turn, s);
+            bound_in_list<true>(listed, [&](int j, uint32_t& key, unsigned long long& mass) { key = s.w[j]; mass = fixed_of(__uint_as_float(key)); return true; },
+                                threshold, hi, [&](unsigned long long all) { return needed_mass(c.p, c.by_count ? all : row_mass); }, turn, s);
+            // Whether the row's mass in integers says the same.  The sum is off by less than 2^-17 of it and 2^-40 a token: with A = -log2 w a weight's argument is off by
+            // 0.69 A 2^-22 here and 0.69 A 2^-23 there, and the mean of A over a mass of 1 and more in N tokens is at most log2 N <= 23 (an entropy); exponentials by
+            // 2^-21 together; a thread's sum takes 10 roundings of 2^-24, and an integer cuts off 2^-40.
+            const unsigned long long doubt = (s.need >> 17) + static_cast<unsigned>(vocab);
+            sure = !c.sums_mass || (s.above + doubt < s.need && s.need + doubt <= s.above + s.within);
         }
         threshold = max(threshold, __float_as_uint(c.least));
         // in the order of the tokens: the greatest of the numbers counted from the row's end
@@ -393,35 +411,39 @@ __device__ __forceinline__ void pick_of_row(const float* __restrict__ row, int v
             mass = fixed_of(__uint_as_float(s.w[j]));
             return s.w[j] >= threshold;
         };
-        bound_in_list(listed, kept, lo, hi, [&](unsigned long long all) { return drawn_point(c.u, all) + 1ull; }, turn, s);
+        bound_in_list<false>(listed, kept, lo, hi, [&](unsigned long long all) { return drawn_point(c.u, all) + 1ull; }, turn, s);
         for (int j = threadIdx.x; j < listed; j += kSampleThreads) {
             uint32_t key;
             unsigned long long mass;
             if (kept(j, key, mass) && key >= lo && key < hi) *out = s.token[j];       // (one token, the most likely ones being kept)
         }
-    } else {
-        auto each = [&](auto f) {
-            for_each_in_row<4>(row, vocab, threadIdx.x, kSampleThreads, [&](int j, float x) { f(j, x <= mx ? weight_of(x, mx, inv_t) : 0.f); });
-        };
+        // (asked behind the draw: with a branch around it 1,024 rows of 32,768 took 31.0 us, 29.9 so)
+        if (sure) return;
         __syncthreads();
-        if (c.by_count) threshold = select_by_count(each, static_cast<unsigned int>(c.k), s.hist, &s.lo, &s.needed);
-        if (c.by_mass) {
-            unsigned long long mine = 0ull;
-            each([&](int, float w) {
-                if (__float_as_uint(w) >= threshold) mine += fixed_of(w);
-            });
-#pragma unroll
-            for (int o = kWave / 2; o > 0; o >>= 1) mine += __shfl_xor(mine, o, kWave);
-            if (lane == 0) s.sums[wave] = mine;
-            __syncthreads();
-            unsigned long long all = 0ull;
-            for (int i = 0; i < kWaves; ++i) all += s.sums[i];
-            __syncthreads();
-            threshold = select_by_mass(each, threshold, 0x3f800001u, 0ull, needed_mass(c.p, all), s.sums, &s.lo, &s.hi, &s.above);
-        }
-        const int picked = draw_from_row(row, vocab, mx, inv_t, max(threshold, __float_as_uint(c.least)), c.u, s);
-        if (threadIdx.x == 0) *out = picked;
     }
+    // a list without room or bounds, or one whose border is in doubt: the row is walked
+    threshold = 0u;
+    auto each = [&](auto f) {
+        for_each_in_row<4>(row, vocab, threadIdx.x, kSampleThreads, [&](int j, float x) { f(j, x <= mx ? weight_of(x, mx, inv_t) : 0.f); });
+    };
+    __syncthreads();
+    if (c.by_count) threshold = select_by_count(each, static_cast<unsigned int>(c.k), s.hist, &s.lo, &s.needed);
+    if (c.by_mass) {
+        unsigned long long mine = 0ull;
+        each([&](int, float w) {
+            if (__float_as_uint(w) >= threshold) mine += fixed_of(w);
+        });
+#pragma unroll
+        for (int o = kWave / 2; o > 0; o >>= 1) mine += __shfl_xor(mine, o, kWave);
+        if (lane == 0) s.sums[wave] = mine;
+        __syncthreads();
+        unsigned long long all = 0ull;
+        for (int i = 0; i < kWaves; ++i) all += s.sums[i];
+        __syncthreads();
+        threshold = select_by_mass(each, threshold, 0x3f800001u, 0ull, needed_mass(c.p, all), s.sums, &s.lo, &s.hi, &s.above);
+    }
+    const int picked = draw_from_row(row, vocab, mx, inv_t, max(threshold, __float_as_uint(c.least)), c.u, s);
+    if (threadIdx.x == 0) *out = picked;
 }
 
 // A row that one workgroup's registers hold.

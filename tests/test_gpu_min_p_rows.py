@@ -114,3 +114,29 @@ def test_a_neighbour_with_min_p_costs_its_own_time(monkeypatch, top_k, top_p):
 def test_mixed_calls_are_refused_without_min_p():
     with pytest.raises(ValueError):
         kernels.backend().sample(torch.zeros((2, 9), device=DEV), *operands(2, 1.0, 0, 1.0, 0.1)[:5], mixed=True)
+
+
+@pytest.mark.parametrize("vocab", [700, 5000, 32766, 40000, 151936])
+def test_tokens_on_the_border_of_top_p_are_kept_by_the_exact_mass(monkeypatch, vocab):
+    # Logits that fall along the row, a top_p that is the running share of one of them to the last bits, and a draw of the last token that is kept: which one that is follows
+    # from sums in integers, as the kernels without min-p have it, however the row is cut.  (A min_p below all of those tokens.)
+    rows, g = 192, torch.Generator().manual_seed(vocab)
+    x = torch.sort(torch.randn((rows, vocab), generator=g) * 2.5, descending=True).values.to(DEV)
+    w = torch.exp(x - x[:, :1]).double()
+    share = torch.cumsum(w, 1) / w.sum(1, keepdim=True)
+    last = (w >= 2e-3).sum(1)
+    at = (torch.rand((rows,), generator=g).to(DEV) * (last - 1)).long()
+    top_p = share.gather(1, at[:, None])[:, 0].float()
+    k = kernels.backend()
+    temperature, top_k, _, u, out, min_p = operands(rows, 1.0, 0, 1.0, 1e-3)
+    u.fill_(0.99999994)
+    k.sample(x, temperature, top_k, top_p, u, out)
+    want = out.tolist()
+    assert sum(abs(a - b) <= 1 for a, b in zip(want, at.tolist())) == rows
+    for pieces in (None, 3, 8, 17) if vocab < 32769 else (None, 5, 8, 17, 40) if vocab > 100000 else (None, 3, 8, 17):
+        with monkeypatch.context() as m:
+            if pieces is not None and vocab > 1024:
+                m.setattr(k, "_sample_pieces", lambda *a: pieces, raising=False)
+            k.sample(x, temperature, top_k, top_p, u, out, min_p=min_p)
+        got = out.tolist()
+        assert [(r, a, b) for r, (a, b) in enumerate(zip(got, want)) if a != b] == [], pieces
