@@ -9,9 +9,9 @@
 // A row in pieces leaves a list, a maximum and a mass for each, and a second kernel joins them: the pieces' bounds are lower than the row's, so their
 // lists hold what the row's does.  Rows that leave too long a list (nearly flat ones; top-p alone with a min_p of 0) are walked again for each threshold.
 //
-// What bounds it: for many rows the one pass over the logits (1,024 rows of 32,768 with top-p and min-p: 29.7 us, 4.5 TB/s, where a copy reaches 5.1;
+// What bounds it: for many rows the one pass over the logits (1,024 rows of 32,768 with top-p and min-p: 30.1 us, 4.5 TB/s, where a copy reaches 5.1;
 // 254 by the kernels that count and list in passes of their own, with a workgroup's list of hundreds compared pair by pair); for a few the chain of a load, a
-// dozen barriers and a second launch (1 row of 151,936 7.8 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 19.2).
+// dozen barriers and a second launch (1 row of 151,936 7.9 us, where an almost empty row of 650 takes 6.6 by one launch; 64 rows with all three cuts 19.4).
 // Rows without a usable bound: 64 of 151,936 with top-p alone 263 us, a min_p of 10^-6 45.
 #include "api.h"
 #include "common.h"
